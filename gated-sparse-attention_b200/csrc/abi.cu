@@ -44,6 +44,13 @@ static int device_info(DeviceInfo* out) {
   return GSA_OK;
 }
 
+int device_error_word(int** err) {
+  DeviceInfo di;
+  const int st = device_info(&di);
+  if (st == GSA_OK) *err = di.err;
+  return st;
+}
+
 static bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Query chunks of at most ``rows`` rows for the indexer passes.  Lq <= rows: whole sequences,

@@ -12,6 +12,9 @@ inline bool dims_ok(const gsa_dims* d) {
          d->d_head > 0 && d->d_head % 2 == 0 && d->n_idx_heads > 0 && d->d_idx > 0;
 }
 
+// Address of the device's error word in the current context (abi.cu).
+int device_error_word(int** err);
+
 struct EpiArgs {
   gsa_dims d;
   gsa_proj_layout lay;

@@ -28,6 +28,17 @@ from .models import (
     RMSNorm,
 )
 
+from .ops import PackedActivation
+from .training import (
+    apply_rotary,
+    fused_next_token_loss,
+    pack_activation,
+    packed_add_rmsnorm,
+    packed_mlp_block,
+    packed_silu_mul,
+    rotary_frequencies,
+)
+
 __version__ = "0.1.0"
 __all__ = [
     "GSAConfig",
@@ -47,4 +58,12 @@ __all__ = [
     "GSALlamaModel",
     "GSALlamaForCausalLM",
     "GSAForCausalLM",
+    "rotary_frequencies",
+    "apply_rotary",
+    "PackedActivation",
+    "pack_activation",
+    "packed_add_rmsnorm",
+    "packed_silu_mul",
+    "packed_mlp_block",
+    "fused_next_token_loss",
 ]

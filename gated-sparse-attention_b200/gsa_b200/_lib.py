@@ -46,6 +46,11 @@ class ProjLayout(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("q", "k", "v", "g2", "g1", "qi", "ki", "wi")]
 
 
+class RotarySide(C.Structure):
+    _fields_ = ([("in_", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32)]
+                + [(n, C.c_int64) for n in ("in_b", "in_l", "in_h", "out_b", "out_l", "out_h")])
+
+
 class TopkParams(C.Structure):
     _fields_ = [("k_base", C.c_int32), ("k_min", C.c_int32), ("k_max", C.c_int32),
                 ("use_adaptive", C.c_int32), ("temperature", C.c_float)]
@@ -100,10 +105,21 @@ SIGNATURES = {
     "gsa_proj_fused_rows": [P],
     "gsa_proj_fused": [P, INT, I64, I64, P, I64, P, P, P, I64, P, P, INT, I64, P, P, P, I64, I64, P, P, I64, P, I64,
                        I64, P, P, P],
+    "gsa_rotary": [INT, I64, I64, I32, I32, P, P, P, I64, I64, P, P, P, INT, I64, I64, F32, INT, INT, P],
+    "gsa_pack_e4m3": [INT, I64, I64, P, I64, P, I64, P, I64, P],
+    "gsa_unpack_e4m3": [INT, I64, I64, P, I64, P, I64, P, I64, P],
+    "gsa_silu_mul_pack": [INT, I64, I64, P, I64, P, I64, P, I64, P, I64, P],
+    "gsa_silu_mul_packed_backward": [INT, I64, I64, P, I64, P, I64, P, I64, P, I64, P, I64, P],
+    "gsa_add_rmsnorm_pack": [INT, I64, I64, P, I64, P, I64, P, F32, P, I64, P, I64, P, I64, P, I64, P, P],
+    "gsa_rmsnorm_packed_workspace_size": [I64, I64],
+    "gsa_rmsnorm_packed_backward": [INT, I64, I64, P, I64, P, I64, P, P, I64, P, I64, P, P, I64, P, I64, P, P, I64, P],
+    "gsa_next_token_loss": [INT, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, P, P, I64, I64, P],
+    "gsa_scale": [INT, I64, P, P, P],
 }
 _RESTYPES = {"gsa_version": C.c_char_p, "gsa_workspace_size": C.c_int64,
              "gsa_survivors_workspace_size": C.c_int64, "gsa_sdpa_workspace_size": C.c_int64,
              "gsa_survivors_fused_workspace_size": C.c_int64,
+             "gsa_rmsnorm_packed_workspace_size": C.c_int64,
              "gsa_decode_workspace_size": C.c_int64, "gsa_proj_fused_rows": C.c_int64}
 
 _lib = None

@@ -329,6 +329,88 @@ int gsa_silu_mul(int dtype, int64_t T, int64_t n, const void* gu, int64_t gu_ld,
                  int64_t z_ld, gsa_stream_t stream);
 
 /*
+ * Rotary positions on q and k (RotaryEmbedding / apply_rotary_pos_emb, rope.py:117-185, with the angles in 64
+ * bits, both pair layouts and rotation of a part of the head): on the first rd of D values of every head
+ *   y0 = x0 c - x1 s, y1 = x1 c + x0 s,  c = factor cos(p f_i), s = factor sin(p f_i)
+ * with the pairs (x_i, x_{i+rd/2}), or (x_{2i}, x_{2i+1}) when interleaved; inverse: s -> -s (the backward pass).
+ * The other D - rd values are copied.
+ *   q, k       gsa_rotary_side of [B, L, heads, D] tensors with contiguous values; strides in elements (input
+ *              strides may be 0); in == out with the same strides rotates in place, otherwise the two must not
+ *              overlap; k may be NULL.  At most 1024 heads together, D <= 1024.
+ *   positions  int64, element (b, l) at b * pos_bstride + l * pos_lstride (0: shared)
+ *   inv_freq   [rd/2] fp64 f_i, or NULL: c and s from cos_tab / sin_tab [tab_rows, >= rd/2] (row stride tab_ld,
+ *              tab_dtype) times factor; a position outside the tables gives NaN and GSA_ERR_INDEX.
+ */
+typedef struct {
+  const void* in;
+  void* out;
+  int32_t heads;
+  int64_t in_b, in_l, in_h, out_b, out_l, out_h;
+} gsa_rotary_side;
+int gsa_rotary(int dtype, int64_t B, int64_t L, int32_t D, int32_t rd, const gsa_rotary_side* q,
+               const gsa_rotary_side* k, const int64_t* positions, int64_t pos_bstride, int64_t pos_lstride,
+               const double* inv_freq, const void* cos_tab, const void* sin_tab, int tab_dtype,
+               int64_t tab_ld, int64_t tab_rows, float factor, int interleaved, int inverse,
+               gsa_stream_t stream);
+
+/*
+ * Activations in 8 bits for the backward pass.  A packed row of n values holds n e4m3 codes (row stride c_ld, a
+ * multiple of 16 and at least n rounded up to 16; the base 16-byte aligned) and a scale byte for each
+ * group of 32 (row stride s_ld >= ceil(n / 32)): byte s stands for 2^(s - 127), the least power of two (s >= 0) that
+ * brings the group's largest finite magnitude to at most 448; codes are rounded to nearest even; NaN
+ * and infinities become NaN (a magnitude of 1.9375 * 2^127 or more rounds to 2^128, which unpacks as
+ * infinity).  Codes of positions n .. c_ld - 1 are not specified.
+ *   gsa_pack_e4m3 / gsa_unpack_e4m3   x [rows, n] <-> packed rows
+ *   gsa_silu_mul_pack                 z = silu(g) * u with g = gu[:, :n], u = gu[:, n:2n] (GSAMlp,
+ *                                     gsa_llama.py:45-46); packed rows 2r, 2r + 1 = g, u of row r
+ *   gsa_silu_mul_packed_backward      dgu (and z again, nullable) from dz and the packed g, u
+ *   gsa_add_rmsnorm_pack              h = x + a in the dtype (a nullable: h = x, h_out then NULL; h_out
+ *                                     nullable), rstd = 1 / sqrt(mean h^2 + eps) [rows] fp32,
+ *                                     y = h * rstd * weight, h packed (RMSNorm, gsa_llama.py:18-30)
+ *   gsa_rmsnorm_packed_backward       from the packed h and rstd: dx = rstd * (dy * w - xh * mean(dy * w * xh)) (+ dh,
+ *                                     nullable) with xh = h * rstd; y = xh * w (nullable); dw = sum over rows of
+ *                                     dy * xh in the dtype (nullable; needs a workspace of
+ *                                     gsa_rmsnorm_packed_workspace_size(rows, d) bytes, 16-byte aligned).  The sums
+ *                                     run in a fixed order.  rows = 0 sets dw to 0.
+ * Inputs may have row strides below n (0: a broadcast row); outputs may not overlap anything.
+ */
+int gsa_pack_e4m3(int dtype, int64_t rows, int64_t n, const void* x, int64_t x_ld, uint8_t* codes,
+                  int64_t c_ld, uint8_t* scales, int64_t s_ld, gsa_stream_t stream);
+int gsa_unpack_e4m3(int dtype, int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld,
+                    const uint8_t* scales, int64_t s_ld, void* x, int64_t x_ld, gsa_stream_t stream);
+int gsa_silu_mul_pack(int dtype, int64_t rows, int64_t n, const void* gu, int64_t gu_ld, void* z,
+                      int64_t z_ld, uint8_t* codes, int64_t c_ld, uint8_t* scales, int64_t s_ld,
+                      gsa_stream_t stream);
+int gsa_silu_mul_packed_backward(int dtype, int64_t rows, int64_t n, const void* dz, int64_t dz_ld,
+                                 const uint8_t* codes, int64_t c_ld, const uint8_t* scales, int64_t s_ld,
+                                 void* dgu, int64_t dgu_ld, void* z, int64_t z_ld, gsa_stream_t stream);
+int gsa_add_rmsnorm_pack(int dtype, int64_t rows, int64_t d, const void* x, int64_t x_ld, const void* a,
+                         int64_t a_ld, const void* weight, float eps, void* h, int64_t h_ld, void* y,
+                         int64_t y_ld, uint8_t* codes, int64_t c_ld, uint8_t* scales, int64_t s_ld,
+                         float* rstd, gsa_stream_t stream);
+int64_t gsa_rmsnorm_packed_workspace_size(int64_t rows, int64_t d);
+int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* dy, int64_t dy_ld,
+                                const void* dh, int64_t dh_ld, const void* weight, const uint8_t* codes,
+                                int64_t c_ld, const uint8_t* scales, int64_t s_ld, const float* rstd,
+                                void* dx, int64_t dx_ld, void* y, int64_t y_ld, void* dw, void* workspace,
+                                int64_t workspace_bytes, gsa_stream_t stream);
+
+/*
+ * Next-token loss with its gradient (GSALlamaForCausalLM.forward, gsa_llama.py:323-336): position (b, t) of
+ * logits [B, L, V] predicts labels[b, t + 1]; the last position, and labels equal to ignore_index, do not count.
+ *   loss [1] fp32 = mean over the counted positions of (log sum exp(x) - x[label]); NaN if none counts
+ *   grad (nullable) [B, L, V] dtype = (softmax(x) - onehot(label)) / count; 0 in positions that do not count
+ *   row_loss [B * L] fp32: each position's loss (0 where it does not count)
+ * Logits of -inf have probability 0.  A counted label outside [0, V) gives NaN and GSA_ERR_INDEX.
+ * gsa_scale: x[0 .. n) *= *factor (a device scalar; 1 leaves x unread).
+ */
+int gsa_next_token_loss(int dtype, int64_t B, int64_t L, int64_t V, const void* logits, int64_t x_bstride,
+                        int64_t x_lstride, const int64_t* labels, int64_t lab_bstride, int64_t lab_lstride,
+                        int64_t ignore_index, float* row_loss, float* loss, void* grad, int64_t g_bstride,
+                        int64_t g_lstride, gsa_stream_t stream);
+int gsa_scale(int dtype, int64_t n, void* x, const float* factor, gsa_stream_t stream);
+
+/*
  * Workspace for gsa_indexer_select: bytes needed for a query chunk of ``chunk_rows`` rows
  * against n_cols keys.
  */

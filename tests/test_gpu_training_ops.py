@@ -1,0 +1,656 @@
+"""The training-step operators (rotary positions, activations in 8 bits with the norm and SwiGLU that use them, the
+next-token loss) against their formulas in 64 bits.
+
+Tolerances count roundings: an output of type t is off by at most half a step of it (eps/2 of its size) plus what the 32-bit
+arithmetic before that rounding loses (each test derives it).  Packed values are compared for equality: the
+scale is a power of two, so the one rounding of a value is the same in any arithmetic."""
+
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+U = 2.0 ** -24  # half a step of fp32, relative
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _randn(seed, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, device=DEV, generator=_gen(seed)) * scale).to(dtype)
+
+
+def _half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _near(got, want, slack, what=""):
+    """|got - want| <= half a step of got's type at want + slack (a tensor or number), elementwise."""
+    bound = _half_step(got.dtype) * (want.abs() + slack) + slack + torch.finfo(got.dtype).tiny
+    off = (got.double() - want).abs() - bound
+    assert got.shape == want.shape, (what, got.shape, want.shape)
+    assert not bool(torch.isnan(off).any()) and float(off.max() if off.numel() else 0) <= 0, (
+        what, float(off.max()), int(off.argmax()))
+
+
+# -- rotary -------------------------------------------------------------------------------------
+def _rotary_oracle(x, positions, freq, factor, interleaved, inverse=False):
+    """x [B, L, H, D] turned in 64 bits, and |x0| + |x1| of each value's pair."""
+    rd = 2 * freq.numel()
+    ang = positions.double().view(-1, x.shape[1], 1, 1) * freq
+    c, s = factor * ang.cos(), factor * ang.sin() * (-1 if inverse else 1)
+    y, size = x.double().clone(), torch.zeros_like(x, dtype=torch.float64)
+    i = torch.arange(rd // 2, device=x.device)
+    i0, i1 = (2 * i, 2 * i + 1) if interleaved else (i, i + rd // 2)
+    x0, x1 = x.double()[..., i0], x.double()[..., i1]
+    y[..., i0], y[..., i1] = x0 * c - x1 * s, x1 * c + x0 * s
+    size[..., i0] = size[..., i1] = x0.abs() + x1.abs()
+    return y, size
+
+
+ROTARY = [
+    # B, L, H, Hk, D, rd, interleaved
+    (1, 1, 1, 1, 2, 2, False),
+    (64, 1, 32, 8, 128, 128, False),
+    (2, 77, 8, 2, 64, 64, False),
+    (2, 33, 32, 8, 128, 64, True),
+    (3, 19, 9, 3, 80, 80, False),
+    (3, 19, 9, 3, 80, 20, True),
+    (1, 65, 5, 1, 96, 34, False),
+    (1, 7, 3, 1, 10, 6, True),
+    (1, 5, 2, 2, 33, 2, False),
+    (1, 40, 16, 16, 256, 256, True),
+    (1, 3, 1000, 24, 16, 16, False),
+    (1, 3, 2, 1, 1024, 1024, False),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,Hk,D,rd,interleaved", ROTARY)
+def test_rotary_forward_and_backward(cuda_ok, dtype, B, L, H, Hk, D, rd, interleaved):
+    import gsa_b200 as gsa
+
+    q, k = _randn(1, B, L, H, D, dtype=dtype), _randn(2, B, L, Hk, D, dtype=dtype)
+    pos = torch.randint(0, 1 << 20, (B, L), device=DEV, generator=_gen(3))
+    freq, factor = gsa.rotary_frequencies(rd, scaling=dict(type="linear", factor=2.0, attention_factor=1.25),
+                                          device=DEV)
+    q.requires_grad_(True)
+    k.requires_grad_(True)
+    q2, k2 = gsa.apply_rotary(q, k, pos, freq, factor, interleaved)
+    dq, dk = _randn(4, B, L, H, D, dtype=dtype), _randn(5, B, L, Hk, D, dtype=dtype)
+    gq, gk = torch.autograd.grad((q2, k2), (q, k), (dq, dk))
+    # sine and cosine of a 32-bit fraction of a turn: pi U each from the fraction's rounding, 2 steps from the function,
+    # the product with the factor, a product and a sum: under 12 U of factor (|x0| + |x1|)
+    for got, x, inv in ((q2, q, False), (k2, k, False), (gq, dq, True), (gk, dk, True)):
+        want, size = _rotary_oracle(x.detach(), pos, freq, factor, interleaved, inv)
+        _near(got.detach(), want, 12 * U * factor * size)
+    # the pass-through part is copied bit for bit
+    assert torch.equal(q2.detach()[..., rd:], q.detach()[..., rd:])
+
+
+def test_rotary_gradient_is_that_of_differences(cuda_ok):
+    """<R x, g> differenced in x against the backward pass: R is linear, so any step gives it, to 32-bit rounding."""
+    import gsa_b200 as gsa
+
+    q = _randn(1, 1, 6, 2, 16).requires_grad_(True)
+    freq, _ = gsa.rotary_frequencies(8, device=DEV)
+    pos = torch.arange(6, device=DEV) * 1000
+    g = _randn(2, 1, 6, 2, 16)
+    y, _ = gsa.apply_rotary(q, None, pos, freq, interleaved=True)
+    (grad,) = torch.autograd.grad(y, q, g)
+    v = _randn(3, 1, 6, 2, 16)
+    with torch.no_grad():
+        up = gsa.apply_rotary(q + v, None, pos, freq, interleaved=True)[0].double()
+        down = gsa.apply_rotary(q - v, None, pos, freq, interleaved=True)[0].double()
+    diff = float(((up - down) / 2 * g.double()).sum())
+    # 192 terms, each of size about 1, off by under 16 U
+    assert abs(diff - float((grad.double() * v.double()).sum())) < 192 * 16 * U * 8
+
+
+def test_rotary_layouts_strides_and_outputs(cuda_ok):
+    """Slices of a fused projection, [B, H, L, D] storage, shared and int32 positions, cache slots, in place, only q,
+    a gradient for one of the two, expanded gradients."""
+    import gsa_b200 as gsa
+
+    B, L, H, Hk, D = 2, 21, 4, 2, 64
+    freq, _ = gsa.rotary_frequencies(D, device=DEV)
+    pos = torch.randint(0, 4096, (L,), device=DEV, generator=_gen(1))
+    proj = _randn(2, B, L, (H + 2 * Hk) * D + 3, dtype=torch.bfloat16)
+    q = proj[..., 1:1 + H * D].view(B, L, H, D)      # rows at odd element offsets
+    k = proj[..., 1 + H * D:1 + (H + Hk) * D].view(B, L, Hk, D)
+    want_q, _ = gsa.apply_rotary(q.contiguous(), None, pos, freq)
+    want_k, _ = gsa.apply_rotary(k.contiguous(), None, pos, freq)
+    got = gsa.apply_rotary(q, k, pos.int(), freq)
+    assert torch.equal(got[0], want_q) and torch.equal(got[1], want_k)
+    # heads before tokens in memory, and a stride between values
+    qt = q.transpose(1, 2).contiguous().transpose(1, 2)
+    assert torch.equal(gsa.apply_rotary(qt, k, pos.view(1, L), freq)[0], want_q)
+    wide = torch.empty(B, L, H, 2 * D, device=DEV, dtype=torch.bfloat16)
+    wide[..., ::2] = q
+    assert torch.equal(gsa.apply_rotary(wide[..., ::2], None, pos, freq)[0], want_q)
+    # K into the slots of a cache, its neighbours left as they were
+    kv = torch.full((B, L + 9, 2, Hk, D), 7.0, device=DEV, dtype=torch.bfloat16)
+    slot = kv[:, 4:4 + L, 0]
+    out = gsa.apply_rotary(q, k, pos, freq, out=(torch.empty_like(want_q), slot))
+    assert out[1].data_ptr() == slot.data_ptr() and torch.equal(slot, want_k)
+    assert bool((kv[:, :4] == 7).all() and (kv[:, 4 + L:] == 7).all() and (kv[:, :, 1] == 7).all())
+    # in place, inside the projection
+    keep = proj.clone()
+    gsa.apply_rotary(q, k, pos, freq, out=(q, k))
+    assert torch.equal(q, want_q) and torch.equal(k, want_k)
+    assert torch.equal(proj[..., (H + Hk) * D + 1:], keep[..., (H + Hk) * D + 1:])
+    assert torch.equal(proj[..., 0], keep[..., 0])
+    # in place with a part of the head: the rest is not written
+    half, _ = gsa.rotary_frequencies(16, device=DEV)
+    x = _randn(5, 1, 3, 2, D)
+    y = gsa.apply_rotary(x, None, pos[:3], half)[0]
+    gsa.apply_rotary(x, None, pos[:3], half, out=(x, None))
+    assert torch.equal(x, y)
+    # gradients: k alone, and an expanded one
+    q32, k32 = _randn(6, B, L, H, D).requires_grad_(True), _randn(7, B, L, Hk, D).requires_grad_(True)
+    q2, k2 = gsa.apply_rotary(q32, k32, pos, freq)
+    (gk,) = torch.autograd.grad(k2.sum(), k32, retain_graph=True)
+    want, size = _rotary_oracle(torch.ones_like(k32), pos.view(1, L), freq, 1.0, False, True)
+    _near(gk, want, 12 * U * size)
+    gq, gk2 = torch.autograd.grad(q2.sum(), (q32, k32), allow_unused=True)
+    assert gk2 is None and bool(torch.isfinite(gq).all())
+    # a broadcast head: its gradient is the sum over the places it stands in
+    one = _randn(8, B, L, 1, D).requires_grad_(True)
+    y = gsa.apply_rotary(one.expand(B, L, H, D), None, pos, freq)[0]
+    g = _randn(9, B, L, H, D)
+    (g1,) = torch.autograd.grad(y, one, g)
+    want, size = _rotary_oracle(g, pos.view(1, L), freq, 1.0, False, True)
+    _near(g1, want.sum(2, keepdim=True), (12 + H) * U * size.sum(2, keepdim=True))
+
+
+def test_rotary_far_positions_and_tables(cuda_ok):
+    """Positions past 2^31 keep their angle; the tables of RotaryEmbedding give torch's bits for its transpose; a position
+    outside the tables is reported and gives NaN."""
+    import gsa_b200 as gsa
+    from gsa_b200 import _lib, ops
+    from gsa_b200.attention import _rope_backward
+
+    freq, _ = gsa.rotary_frequencies(64, device=DEV)
+    x = _randn(1, 1, 8, 3, 64)
+    pos = torch.tensor([0, 1, 131071, 1 << 20, (1 << 31) + 5, 1 << 33, -3, 12345678901], device=DEV).view(1, 8)
+    y, _ = gsa.apply_rotary(x, None, pos, freq)
+    want, size = _rotary_oracle(x, pos, freq, 1.0, False)
+    # the 64-bit angle itself is off by up to p 2^-53 on either side: 2^34 2^-52 = 2^-18 for the largest
+    _near(y, want, size * (12 * U + 2.0 ** -52 * pos.abs().double().view(1, 8, 1, 1)))
+    for dt in (torch.float32, torch.bfloat16):
+        emb = gsa.RotaryEmbedding(64, 512).to(DEV).to(dt)
+        p = torch.randint(0, 512, (2, 8), device=DEV, generator=_gen(4))
+        dy = _randn(5, 2, 8, 3, 64)
+        want = _rope_backward(dy.view(16, 3, 64), emb.cos_cached[p.view(-1)], emb.sin_cached[p.view(-1)])
+        got, _ = ops.rotary(dy, None, p, tables=(emb.cos_cached, emb.sin_cached), rotary_dim=64, inverse=True)
+        assert torch.equal(got.view(16, 3, 64), want)
+    p[1, 3] = 512
+    got, _ = ops.rotary(dy, None, p, tables=(emb.cos_cached, emb.sin_cached), rotary_dim=64)
+    assert bool(torch.isnan(got[1, 3]).all()) and not bool(torch.isnan(got[0]).any())
+    with pytest.raises(_lib.GSAError):
+        ops.check_device_error()
+    ops.check_device_error()
+
+
+def test_rotary_empty_inputs(cuda_ok):
+    import gsa_b200 as gsa
+
+    freq, _ = gsa.rotary_frequencies(8, device=DEV)
+    for B, L in ((0, 5), (2, 0)):
+        q = torch.empty(B, L, 2, 8, device=DEV)
+        y, k = gsa.apply_rotary(q, q, torch.zeros(B, L, device=DEV, dtype=torch.long), freq)
+        assert y.shape == q.shape and k.shape == q.shape
+
+
+# -- 8 bits -------------------------------------------------------------------------------------
+def _eight(x):
+    """x [..., n] (64 bits) as 8 bits hold it, by the definition: per group of 32 the least e >= -127 with
+    max finite |x| <= 448 2^e, each value to the nearest of e4m3's multiples (ties to even); NaN for NaN and inf."""
+    n = x.shape[-1]
+    g = torch.nn.functional.pad(x, (0, -n % 32)).unflatten(-1, (-1, 32))
+    top = torch.where(torch.isfinite(g), g.abs(), 0.0).amax(-1, keepdim=True)
+    e = torch.full_like(top, -127.0)
+    for cand in range(120, -128, -1):  # the last candidate that still holds the group is the least
+        e = torch.where(top <= 448 * 2.0 ** cand, torch.full_like(e, cand), e)
+    v = g / torch.exp2(e)
+    ex = torch.frexp(torch.where(torch.isfinite(v), v, 0.0))[1] - 1
+    step = torch.exp2(ex.clamp(min=-6).double() - 3)
+    q = torch.where(torch.isfinite(v), torch.round(v / step) * step, math.nan) * torch.exp2(e)
+    return q.flatten(-2)[..., :n], e.squeeze(-1)
+
+
+def _same(a, b):
+    return bool(((a == b) | (torch.isnan(a) & torch.isnan(b))).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(1, 1), (5, 31), (4, 32), (3, 33), (2, 7, 48), (3, 1000), (17, 4096), (2, 11008), (1000, 16),
+                                   (7, 160), (9,)])
+def test_pack_and_unpack_are_the_definition(cuda_ok, dtype, shape):
+    import gsa_b200 as gsa
+
+    x = (_randn(1, *shape) * torch.exp(_randn(2, *shape) * 6)).to(dtype)
+    p = gsa.pack_activation(x)
+    want, e = _eight(x.double())
+    got = p.unpack()
+    assert got.dtype == dtype and got.shape == x.shape
+    assert torch.equal(p.unpack(torch.float32).double(), want)
+    assert torch.equal(p.scales.view(e.shape).double() - 127, e)
+    n = shape[-1]
+    assert p.nbytes == x.numel() // n * ((n + 15) // 16 * 16 + (n + 31) // 32)
+    # what 8 bits promise: within 2^-4 of the value, or 2^-17 of the group's largest (half a step of 2^-9 2^e against more than 224 2^e)
+    big = torch.nn.functional.pad(x.double().abs(), (0, -n % 32)).unflatten(-1, (-1, 32))
+    big = big.amax(-1, keepdim=True).expand_as(big).flatten(-2)[..., :n]
+    assert bool(((want - x.double()).abs() <= torch.maximum(x.double().abs() * 2.0 ** -4, big * 2.0 ** -17)).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [64, 37])
+def test_pack_special_values(cuda_ok, dtype, n):
+    """Zeros, the type's smallest and largest numbers, NaN and infinities beside ordinary values, ties, borders
+    of the scale."""
+    import gsa_b200 as gsa
+
+    rows = []
+    fi = torch.finfo(dtype)
+    for fill in ([0.0], [-0.0], [fi.max], [fi.max, fi.tiny], [fi.tiny], [fi.smallest_normal / 64], [448.0, 2.0 ** -10, 2.0 ** -11],
+                 [449.0, 1.0], [450.0, 17.0, 18.0, 19.0, 21.0], [1.75, 1.0625, 1.1875], [1.7578125, 1.0625],
+                 [math.nan, 1.0], [math.inf, 1.0, 3.0], [-math.inf, math.nan], [math.nan], [2.0 ** -120, 2.0 ** -126],
+                 [-3.5, 2.0 ** -9 * 3.5, 2.0 ** -16 * 3.5, 2.0 ** -20]):
+        rows.append([fill[i % len(fill)] for i in range(n)])
+    x = torch.tensor(rows, dtype=torch.float64).to(dtype).to(DEV)
+    got = gsa.pack_activation(x).unpack(torch.float32).double()
+    # the packed value of the largest numbers is 256 * 2^120 = 2^128, which fp32 holds as infinity
+    want = _eight(x.double())[0].float().double()
+    assert _same(got, want), (got - want).abs().max()
+
+
+def test_pack_strided_and_empty(cuda_ok):
+    import gsa_b200 as gsa
+
+    base = _randn(1, 12, 200, dtype=torch.bfloat16)
+    for x in (base[:, 3:99], base[::2, :96], base.t(), base[:, ::2], base[:1].expand(5, 200), base[:, :64].unflatten(1, (2, 32))):
+        assert torch.equal(gsa.pack_activation(x).unpack(), gsa.pack_activation(x.contiguous()).unpack())
+    for shape in ((0, 64), (4, 0), (2, 0, 32)):
+        p = gsa.pack_activation(torch.empty(shape, device=DEV))
+        assert p.unpack().shape == torch.Size(shape) and p.nbytes == 0
+
+
+ROWS = [(1, 1), (3, 16), (2, 31), (5, 33), (192, 512), (7, 1376), (1, 4096), (33, 1000), (3, 11008), (300, 48)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,n", ROWS)
+def test_swiglu_forward_and_backward(cuda_ok, dtype, rows, n):
+    import gsa_b200 as gsa
+
+    gu = _randn(1, rows, 2 * n, dtype=dtype, scale=2.0)
+    dz = _randn(2, rows, n, dtype=dtype)
+    z, p = gsa.ops.silu_mul_packed(gu)
+    g, u = gu.double()[:, :n], gu.double()[:, n:]
+    # the sigmoid is off by 8 U of itself (exp 2 steps, sum, reciprocal), each product by U
+    _near(z, g * torch.sigmoid(g) * u, 12 * U * (g * u).abs())
+    want, _ = _eight(gu.double().view(rows, 2, n))
+    assert torch.equal(p.unpack(torch.float32).double(), want)
+    dgu, z2 = gsa.ops.silu_mul_packed_backward(dz, p, want_z=True)
+    g, u, d = want[:, 0], want[:, 1], dz.double()
+    sig = torch.sigmoid(g)
+    size = (d * u).abs() * sig * (1 + g.abs())
+    _near(dgu[:, :n], d * u * sig * (1 + g * (1 - sig)), 24 * U * size)
+    _near(dgu[:, n:], d * g * sig, 12 * U * (d * g).abs())
+    _near(z2, g * sig * u, 12 * U * (g * u).abs())
+    none = gsa.ops.silu_mul_packed_backward(dz, p)
+    assert none[1] is None and torch.equal(none[0], dgu)
+    # through autograd
+    leaf = gu.clone().requires_grad_(True)
+    y = gsa.packed_silu_mul(leaf)
+    (grad,) = torch.autograd.grad(y, leaf, dz)
+    assert torch.equal(y.detach(), z) and torch.equal(grad, dgu) and torch.equal(gsa.packed_silu_mul(gu), z)
+
+
+def test_swiglu_gradient_is_that_of_differences(cuda_ok):
+    """At values that 8 bits hold exactly, central differences of the 64-bit formula along a direction."""
+    import gsa_b200 as gsa
+
+    gu = _eight(_randn(1, 4, 96).double())[0]
+    v, dz = _randn(2, 4, 96).double(), _randn(3, 4, 48)
+
+    def f(x):
+        return (torch.nn.functional.silu(x[:, :48]) * x[:, 48:] * dz.double()).sum()
+
+    h = 1e-6
+    diff = float((f(gu + h * v) - f(gu - h * v)) / (2 * h))
+    leaf = gu.float().requires_grad_(True)
+    gsa.packed_silu_mul(leaf).backward(dz)
+    # 384 terms of size about 1 at 32 U, and h^2 of the third derivative
+    assert abs(float((leaf.grad.double() * v).sum()) - diff) < 384 * 32 * U + 1e-8
+
+
+def test_swiglu_extreme_gates(cuda_ok):
+    """Gates far out (sigmoid 0 or 1), infinite and NaN ones."""
+    import gsa_b200 as gsa
+
+    g = torch.tensor([-1e30, -200.0, -88.0, 88.0, 200.0, 1e30, 0.0, -0.0], device=DEV).repeat(4)
+    gu = torch.cat([g, torch.ones(32, device=DEV)]).view(1, 64)
+    z, p = gsa.ops.silu_mul_packed(gu)
+    want = torch.nn.functional.silu(g.double())
+    _near(z[0], want, 12 * U * want.abs())
+    dgu, z2 = gsa.ops.silu_mul_packed_backward(torch.ones(1, 32, device=DEV), p, want_z=True)
+    assert bool(torch.isfinite(dgu).all() and torch.isfinite(z2).all())
+    gu[0, 3], gu[0, 40] = math.nan, math.inf
+    z, p = gsa.ops.silu_mul_packed(gu)
+    dgu, _ = gsa.ops.silu_mul_packed_backward(torch.ones(1, 32, device=DEV), p)
+    assert bool(torch.isnan(z[0, 3])) and bool(torch.isnan(dgu[0, 3])) and bool(torch.isnan(dgu[0, 8]))
+    assert int(torch.isnan(dgu).sum()) <= 4  # and in no other column
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("add", [True, False])
+@pytest.mark.parametrize("rows,d", ROWS + [(2, 16384), (1, 20000), (700, 256), (5, 4112), (2000, 8)])
+def test_norm_forward_and_backward(cuda_ok, dtype, add, rows, d):
+    import gsa_b200 as gsa
+
+    x = _randn(1, rows, d, dtype=dtype, scale=2.0)
+    a = _randn(2, rows, d, dtype=dtype) if add else None
+    w = (1 + 0.2 * _randn(3, d)).to(dtype)
+    eps = 1e-5
+    h, y, p, rstd = gsa.ops.add_rmsnorm_packed(x, a, w, eps)
+    hd = (x.double() + a.double()).to(dtype).double() if add else x.double()
+    assert (h is None) == (not add) and (h is None or torch.equal(h.double(), hd))
+    # a sum of d squares in 32 bits: at most d / 32 + 16 additions follow one another in any lane and the tree
+    lose = (d / 32 + 16) * U
+    r = 1 / torch.sqrt(hd.square().mean(-1, keepdim=True) + eps)
+    assert float((rstd.double() / r.view(-1) - 1).abs().max()) <= lose + 8 * U
+    wd = w.double()
+    want = hd * r * wd
+    _near(y, want, (lose + 12 * U) * want.abs())
+    held, _ = _eight(hd)
+    assert torch.equal(p.unpack(torch.float32).double(), held)
+    dy, dh = _randn(4, rows, d, dtype=dtype), _randn(5, rows, d, dtype=dtype)
+    xh = held * r
+    for extra in (dh, None):
+        dx, dw, y2 = gsa.ops.rmsnorm_packed_backward(dy, p, rstd, w, dh=extra, want_y=extra is not None)
+        dyw = dy.double() * wd
+        along = (dyw * xh).mean(-1, keepdim=True)
+        ref = r * (dyw - xh * along)
+        size = r * (dyw.abs() + xh.abs() * (dyw * xh).abs().mean(-1, keepdim=True))
+        if extra is not None:
+            ref, size = ref + extra.double(), size + extra.double().abs()
+        _near(dx, ref, (3 * lose + 24 * U) * size, "dx")
+        _near(dw, (dy.double() * xh).sum(0), (rows + 16 + lose / U) * U * (dy.double() * xh).abs().sum(0), "dw")
+        if extra is not None:
+            _near(y2, xh * wd, (lose + 12 * U) * (xh * wd).abs(), "y")
+    assert y2 is None
+    assert gsa.ops.rmsnorm_packed_backward(dy, p, rstd, w, want_dw=False)[1] is None
+    # the same sums in the same order every time
+    again = gsa.ops.rmsnorm_packed_backward(dy, p, rstd, w)
+    assert torch.equal(again[1], dw) and torch.equal(again[0], dx)
+
+
+def test_norm_autograd_and_differences(cuda_ok):
+    """packed_add_rmsnorm under autograd at values that 8 bits hold exactly, against central differences of the
+    64-bit formula; h's own gradient, unused outputs, no addend."""
+    import gsa_b200 as gsa
+
+    x = _eight(_randn(1, 3, 64).double())[0]
+    w = 1 + 0.1 * _randn(2, 64)
+    gy, gh = _randn(3, 3, 64), _randn(4, 3, 64)
+    zero = torch.zeros(3, 64, device=DEV)
+
+    def f(x, w):
+        return (x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-5) * w * gy.double()).sum() + (x * gh.double()).sum()
+
+    lx, la, lw = x.float().requires_grad_(True), zero.requires_grad_(True), w.clone().requires_grad_(True)
+    h, y = gsa.packed_add_rmsnorm(lx, la, lw, 1e-5)
+    torch.autograd.backward((h, y), (gh, gy))
+    assert torch.equal(lx.grad, la.grad)
+    vx, vw, e = _randn(5, 3, 64).double(), _randn(6, 64).double(), 1e-6
+    diff = float((f(x + e * vx, w.double() + e * vw) - f(x - e * vx, w.double() - e * vw)) / (2 * e))
+    got = float((lx.grad.double() * vx).sum() + (lw.grad.double() * vw).sum())
+    assert abs(got - diff) < 400 * 64 * U + 1e-7
+    # y alone, h alone, and x alone without an addend
+    h, y = gsa.packed_add_rmsnorm(lx, la, lw, 1e-5)
+    g1 = torch.autograd.grad(y, lx, gy, retain_graph=True)[0]
+    assert torch.equal(torch.autograd.grad(h, lx, gh)[0], gh)
+    h, y = gsa.packed_add_rmsnorm(lx, None, lw, 1e-5)
+    assert h is lx and torch.equal(torch.autograd.grad(y, lx, gy)[0], g1)
+
+
+def test_norm_special_rows(cuda_ok):
+    """Rows of zeros, of one huge value, with NaN, strided rows, a broadcast row, no rows."""
+    import gsa_b200 as gsa
+
+    d = 96
+    x = torch.zeros(5, d, device=DEV)
+    x[1, 7] = 1e18
+    x[2, 3] = math.nan
+    x[3] = _randn(1, d)
+    w = torch.ones(d, device=DEV)
+    h, y, p, rstd = gsa.ops.add_rmsnorm_packed(x, torch.zeros_like(x), w, 1e-5)
+    assert bool((y[0] == 0).all()) and abs(float(rstd[0]) - 1e-5 ** -0.5) < 1e-3
+    assert abs(float(y[1, 7]) - math.sqrt(d)) < 1e-3 and bool(torch.isnan(y[2]).all())
+    dx, dw, _ = gsa.ops.rmsnorm_packed_backward(torch.ones_like(x), p, rstd, w)
+    assert bool(torch.isfinite(dx[[0, 1, 3, 4]]).all()) and bool(torch.isnan(dx[2]).all())
+    base = _randn(2, 6, 2 * d + 1, dtype=torch.bfloat16)
+    wb = torch.ones(d, device=DEV, dtype=torch.bfloat16)
+    xs, as_ = base[:, 1:1 + d], base[:1, d:2 * d].expand(6, d)
+    for got, want in zip(gsa.ops.add_rmsnorm_packed(xs, as_, wb, 1e-5)[:2],
+                         gsa.ops.add_rmsnorm_packed(xs.contiguous(), as_.contiguous(), wb, 1e-5)[:2]):
+        assert torch.equal(got, want)
+    empty = torch.empty(0, d, device=DEV)
+    h, y, p, rstd = gsa.ops.add_rmsnorm_packed(empty, empty, w, 1e-5)
+    dx, dw, _ = gsa.ops.rmsnorm_packed_backward(empty, p, rstd, w)
+    assert y.shape == (0, d) and bool((dw == 0).all())
+
+
+# -- loss ---------------------------------------------------------------------------------------
+def _loss_oracle(logits, labels, ignore=-100):
+    x = logits.double()[:, :-1]
+    t = labels[:, 1:]
+    keep = t != ignore
+    logp = torch.log_softmax(x, -1)
+    at = t.clamp(min=0).unsqueeze(-1)
+    nll = torch.where(keep, -logp.gather(-1, at).squeeze(-1), 0.0)
+    count = keep.sum()
+    p = logp.exp()
+    grad = torch.zeros_like(logits, dtype=torch.float64)
+    grad[:, :-1] = torch.where(keep.unsqueeze(-1), (p - torch.zeros_like(p).scatter(-1, at, 1.0)) / count, 0.0)
+    size = torch.zeros_like(grad)  # |softmax| / count + onehot / count, with the distance from the row's largest
+    size[:, :-1] = (p + torch.zeros_like(p).scatter(-1, at, 1.0)) / count
+    far = (x.amax(-1, keepdim=True) - x).clamp(max=200.0)
+    loss_size = torch.where(keep, x.abs().amax(-1) + nll.abs(), 0.0).sum() / count
+    return nll.sum() / count, grad, size, torch.nn.functional.pad(far, (0, 0, 0, 1)), loss_size
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,V", [(1, 2, 1), (1, 2, 2), (2, 96, 384), (3, 17, 1000), (1, 33, 4097), (2, 5, 128256), (1, 600, 31),
+                                   (1, 3, 32768), (700, 2, 8), (1, 9, 50257)])
+def test_loss_and_gradient(cuda_ok, dtype, B, L, V):
+    import gsa_b200 as gsa
+
+    logits = _randn(1, B, L, V, dtype=dtype, scale=3.0)
+    labels = torch.randint(0, V, (B, L), device=DEV, generator=_gen(2))
+    labels[torch.rand(B, L, device=DEV, generator=_gen(3)) < 0.3] = -100
+    labels[0, 1] = V - 1
+    loss, grad = gsa.ops.next_token_loss(logits, labels)
+    want, g, size, far, loss_size = _loss_oracle(logits, labels)
+    # sum of V exponentials, at most V / 32 + 16 additions after one another; each exponential off by 4 U and by U of its
+    # argument; the loss a difference of numbers of the logits' size
+    lose = (V / 32 + 32) * U
+    _near(loss, want, (lose + 8 * U) * (1 + loss_size))
+    _near(grad, g, size * (lose + (far + 16) * U))
+    leaf = logits.clone().requires_grad_(True)
+    out = gsa.fused_next_token_loss(leaf, labels)
+    out.backward()
+    assert torch.equal(out.detach(), loss) and torch.equal(leaf.grad, grad)
+    assert torch.equal(gsa.fused_next_token_loss(logits, labels), loss)
+    # a scaled loss scales the gradient (by a power of two: exactly)
+    leaf.grad = None
+    (gsa.fused_next_token_loss(leaf, labels) * 0.25).backward()
+    assert torch.equal(leaf.grad, (grad.float() * 0.25).to(dtype))
+
+
+def test_loss_gradient_is_that_of_differences(cuda_ok):
+    import gsa_b200 as gsa
+
+    logits, labels = _randn(1, 2, 5, 40), torch.randint(0, 40, (2, 5), device=DEV, generator=_gen(2))
+    v, e = _randn(3, 2, 5, 40).double(), 1e-6
+    up, down = _loss_oracle(logits.double() + e * v, labels)[0], _loss_oracle(logits.double() - e * v, labels)[0]
+    _, grad = gsa.ops.next_token_loss(logits, labels)
+    assert abs(float((grad.double() * v).sum() - (up - down) / (2 * e))) < 400 * 16 * U
+
+
+def test_loss_special_rows(cuda_ok):
+    """Masked (-inf) logits, a target among them, large and equal logits, rows that do not count, no row that counts, another
+    ignore_index, a label out of range, NaN."""
+    import gsa_b200 as gsa
+    from gsa_b200 import _lib, ops
+
+    V = 70
+    x = _randn(1, 1, 6, V)
+    x[0, 0, 5:60] = -math.inf
+    x[0, 1] = 1000.0
+    x[0, 2] = -1000.0
+    x[0, 3, 1:] = torch.finfo(torch.float32).min
+    labels = torch.tensor([[9, 2, 3, 4, 0, 64]], device=DEV)
+    want, g, size, far, loss_size = _loss_oracle(x, labels)
+    loss, grad = ops.next_token_loss(x, labels)
+    _near(loss, want, 64 * U * (1 + loss_size))
+    _near(grad, g, size * 256 * U)
+    assert bool((grad[0, 0, 5:60] == 0).all()) and bool((grad[0, 5] == 0).all())
+    # the target itself masked: an infinite loss, a finite gradient
+    hit = labels.clone()
+    hit[0, 1] = 30
+    loss, grad = ops.next_token_loss(x, hit)
+    assert float(loss) == math.inf and bool(torch.isfinite(grad).all())
+    # nothing counts
+    for lab, ign in ((torch.full_like(labels, -100), -100), (torch.full_like(labels, 7), 7)):
+        loss, grad = ops.next_token_loss(x, lab, ign)
+        assert bool(torch.isnan(loss)) and bool((grad == 0).all())
+    loss, grad = ops.next_token_loss(x[:, :1], labels[:, :1])
+    assert bool(torch.isnan(loss)) and bool((grad == 0).all())
+    # NaN and +inf stay in their rows
+    for bad in (math.nan, math.inf):
+        y = x.clone()
+        y[0, 1, 3] = bad
+        loss, grad = ops.next_token_loss(y, labels)
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(grad[0, 1]).all())
+        assert bool(torch.isfinite(grad[0, [0, 2, 3, 4, 5]]).all())
+    ops.check_device_error()
+    wrong = labels.clone()
+    wrong[0, 2] = V
+    loss, grad = ops.next_token_loss(x, wrong)
+    assert bool(torch.isnan(loss)) and bool(torch.isnan(grad[0, 1]).all()) and bool(torch.isfinite(grad[0, 0]).all())
+    with pytest.raises(_lib.GSAError):
+        ops.check_device_error()
+    # an ignored label may be anything
+    wrong[0, 2] = 12345678
+    loss, _ = ops.next_token_loss(x, wrong, ignore_index=12345678)
+    assert bool(torch.isfinite(loss))
+    ops.check_device_error()
+
+
+def test_loss_strides_types_and_second_backward(cuda_ok):
+    import gsa_b200 as gsa
+
+    B, L, V = 2, 9, 130
+    wide = _randn(1, B, L + 3, 2 * V + 1, dtype=torch.bfloat16)
+    labels = torch.randint(0, V, (L, B), device=DEV, generator=_gen(2)).t()
+    for x in (wide[:, 2:2 + L, 1:1 + V], wide[:, :L, :2 * V:2], wide[:, :L].transpose(0, 1).contiguous().transpose(0, 1)[..., :V],
+              wide[:1, :L, :V].expand(B, L, V)):
+        a, b = gsa.ops.next_token_loss(x, labels), gsa.ops.next_token_loss(x.contiguous(), labels.contiguous().int())
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1]) and a[1].is_contiguous()
+    leaf = wide[:, :L, :V].clone().requires_grad_(True)
+    loss = gsa.fused_next_token_loss(leaf, labels)
+    loss.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="earlier backward"):
+        loss.backward()
+
+
+# -- streams, graphs ----------------------------------------------------------------------------
+def _step(q, k, pos, freq, x, a, w, gu, logits, labels):
+    import gsa_b200 as gsa
+
+    q2, k2 = gsa.ops.rotary(q, k, pos, freq)
+    h, y, p, rstd = gsa.ops.add_rmsnorm_packed(x, a, w, 1e-5)
+    dx, dw, y2 = gsa.ops.rmsnorm_packed_backward(y, p, rstd, w, dh=h, want_y=True)
+    z, pg = gsa.ops.silu_mul_packed(gu)
+    dgu, z2 = gsa.ops.silu_mul_packed_backward(z, pg, want_z=True)
+    loss, grad = gsa.ops.next_token_loss(logits, labels)
+    return q2, k2, h, y, dx, dw, y2, z, dgu, z2, loss, grad
+
+
+def _step_inputs(seed):
+    import gsa_b200 as gsa
+
+    bf = torch.bfloat16
+    return (_randn(seed, 2, 50, 8, 64, dtype=bf), _randn(seed + 1, 2, 50, 2, 64, dtype=bf),
+            torch.randint(0, 5000, (2, 50), device=DEV, generator=_gen(seed)), gsa.rotary_frequencies(64, device=DEV)[0],
+            _randn(seed + 2, 100, 512, dtype=bf), _randn(seed + 3, 100, 512, dtype=bf), _randn(seed + 4, 512, dtype=bf),
+            _randn(seed + 5, 100, 1024, dtype=bf), _randn(seed + 6, 2, 50, 1000, dtype=bf),
+            torch.randint(0, 1000, (2, 50), device=DEV, generator=_gen(seed)))
+
+
+def test_ops_on_a_side_stream_and_in_two_graphs(cuda_ok):
+    """The same bits on another stream, and from two captured graphs that are replayed on new inputs, at once."""
+    sets = [_step_inputs(10), _step_inputs(30)]
+    want = [_step(*s) for s in sets]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _step(*sets[1])
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[1]))
+    graphs = []
+    for s in sets:
+        held = tuple(t.clone() for t in s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = _step(*held)
+        graphs.append((g, held, out))
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(3):
+        for i, (g, held, _) in enumerate(graphs):
+            for t, v in zip(held, sets[(i + turn) % 2]):
+                t.copy_(v)
+        torch.cuda.synchronize()
+        for st, (g, _, _) in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for i, (_, _, out) in enumerate(graphs):
+            assert all(torch.equal(a, b) for a, b in zip(out, want[(i + turn) % 2])), (turn, i)
+
+
+def test_captured_training_step(cuda_ok):
+    """Forward and backward through autograd, captured and replayed: the eager step's bits."""
+    import gsa_b200 as gsa
+
+    def step(x, w, wl, labels):
+        h, y = gsa.packed_add_rmsnorm(x, None, w, 1e-5)
+        z = gsa.packed_silu_mul(y)
+        loss = gsa.fused_next_token_loss(z @ wl, labels)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w, wl)))
+
+    def leaves():
+        return [_randn(i, *s).requires_grad_(True) for i, s in ((1, (2, 16, 128)), (2, (128,)), (3, (64, 90)))]
+
+    labels = torch.randint(0, 90, (2, 16), device=DEV, generator=_gen(4))
+    want = step(*leaves(), labels)
+    ins = leaves()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*ins, labels)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(*ins, labels)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
