@@ -24,7 +24,7 @@ OBJ_DIR = PKG_ROOT / "_build"
 
 SOURCES = ["abi.cu", "proj_epilogue.cu", "indexer_simt.cu", "indexer_tc.cu", "indexer_decode.cu", "topk.cu",
            "sparse_sdpa.cu", "sparse_sdpa_bwd.cu", "select_static.cu", "decoder.cu", "sdpa_probs.cu", "selftest.cu",
-           "proj_gemm.cu", "rotary.cu", "packed.cu", "lm_loss.cu"]
+           "proj_gemm.cu", "rotary.cu", "packed.cu", "packed_norm.cu", "lm_loss.cu"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -1,16 +1,14 @@
-// Activations kept in 8 bits for the backward pass (the form: packed.cuh), and the two decoder-layer products
-// that use them: the residual add with its RMSNorm, and the SwiGLU product.  All are bound by the bytes
-// that they move.
+// Activations kept in 8 bits for the backward pass (the form: packed.cuh), and the SwiGLU product that keeps its
+// operands so.
 //
 //   pack / unpack   x -> codes, scales -> x^
 //   silu_mul        z = g sigma(g) u, (g, u) kept packed; backward, from the packed g^, u^:
 //                   dg = dz u^ sigma (1 + g^ (1 - sigma)), du = dz g^ sigma, z again for the weight gradient of the
 //                   product that reads it
-//   add_rmsnorm     h = x + a, r = (mean h^2 + eps)^(-1/2), y = h r w, h kept packed with r; backward, with
-//                   x^ = h^ r:  dx = r (dy w - x^ mean(dy w x^)) + dh,  dw = sum_rows dy x^,  y again = x^ w
 //
-// Products, sums and statistics are in 32 bits; an output is rounded once, to its type.  h is rounded to its type
-// before the norm, since the residual stream that the backward pass differentiates is what the tensor holds.
+// Products are in 32 bits; an output is rounded once, to its type.  All are bound by the bytes that they move, so
+// a thread holds 16 neighbouring values (half a group, 32-byte loads and stores, one shuffle for the scale) wherever
+// the rows are whole multiples of that and aligned; rows that are not take a value a lane (a group a warp).
 #include <algorithm>
 
 #include "packed.cuh"
@@ -21,66 +19,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// One group by one warp, a value a lane: its code and the scale byte; returns the code (in the low byte).
-__device__ __forceinline__ uint32_t pack_lane(float x, int* scale) {
-  const int s = scale_byte(__reduce_max_sync(0xffffffffu, finite_abs_bits(x)));
-  *scale = s;
-  return to_e4m3x2(inf_to_nan(x) * inv_pow2_of(s), 0.f) & 0xffu;
-}
-
-__device__ __forceinline__ float unpack_one(uint8_t code, uint8_t scale) {
-  return from_e4m3x2(code).x * pow2_of(scale);
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, int64_t n, const T* x, int64_t x_ld,
-                                                        uint8_t* codes, int64_t c_ld, uint8_t* scales, int64_t s_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t g = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); g < total; g += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = g / groups, i = (g - r * groups) * kGroup + lane;
-    int s;
-    const uint32_t c = pack_lane(i < n ? to_float(x[r * x_ld + i]) : 0.f, &s);
-    if (i < c_ld) codes[r * c_ld + i] = (uint8_t)c;
-    if (lane == 0) scales[r * s_ld + i / kGroup] = (uint8_t)s;
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld,
-                                                          const uint8_t* scales, int64_t s_ld, T* x, int64_t x_ld) {
-  const int64_t total = rows * n;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = e / n, i = e - r * n;
-    x[r * x_ld + i] = from_float<T>(unpack_one(codes[r * c_ld + i], scales[r * s_ld + i / kGroup]));
-  }
-}
-
-__device__ __forceinline__ float sigmoid32(float x) { return 1.0f / (1.0f + expf(-x)); }
-
-// gu rows hold g then u; the packed rows 2r and 2r + 1 are row r's g and u.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(int64_t rows, int64_t n, const T* gu, int64_t gu_ld,
-                                                                 T* z, int64_t z_ld, uint8_t* codes, int64_t c_ld,
-                                                                 uint8_t* scales, int64_t s_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); w < total; w += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = w / groups, i = (w - r * groups) * kGroup + lane;
-    const float g = i < n ? to_float(gu[r * gu_ld + i]) : 0.f;
-    const float u = i < n ? to_float(gu[r * gu_ld + n + i]) : 0.f;
-    if (i < n) z[r * z_ld + i] = from_float<T>(g * sigmoid32(g) * u);
-    int sg, su;
-    const uint32_t cg = pack_lane(g, &sg), cu = pack_lane(u, &su);
-    if (i < c_ld) {
-      codes[2 * r * c_ld + i] = (uint8_t)cg;
-      codes[(2 * r + 1) * c_ld + i] = (uint8_t)cu;
-    }
-    if (lane == 0) {
-      scales[2 * r * s_ld + i / kGroup] = (uint8_t)sg;
-      scales[(2 * r + 1) * s_ld + i / kGroup] = (uint8_t)su;
-    }
-  }
+// sigma(x) = 1 / (1 + e^-x), off by a few units over the whole range, the subnormal tail included (z = g sigma(g) keeps
+// its relative accuracy there).
+__device__ __forceinline__ float sigmoid32(float x) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-x)));
+  return r;
 }
 
 struct SwigluGrad {
@@ -91,13 +35,168 @@ __device__ __forceinline__ SwigluGrad swiglu_grad(float dz, float g, float u) {
   return {dz * u * (sig * (1.0f + g * (1.0f - sig))), dz * silu, silu * u};
 }
 
+// ---------------------------------------------------------------------------------------------
+// 16 values a thread.  A row is cut into 2 ceil(n / 32) halves, so that the two halves of a group are
+// neighbouring lanes; the last may be empty.
+// ---------------------------------------------------------------------------------------------
+struct Cut {
+  int64_t rows, halves, per_row;  // halves: rows * per_row
+  uint64_t magic;
+  int64_t n;
+};
+struct Place {
+  int64_t r, i;
+  bool live;
+};
+__device__ __forceinline__ Place place_of(const Cut& c) {
+  const int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t r = row_of(e, c.magic), i = (e - r * c.per_row) * 16;
+  return {r, i, e < c.halves && i < c.n};
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack16_kernel(const Cut c, const T* x, int64_t x_ld, uint8_t* codes,
+                                                          int64_t c_ld, uint8_t* scales, int64_t s_ld) {
+  const Place p = place_of(c);
+  Half<T> h;
+  h.zero();
+  if (p.live) h.load(x + p.r * x_ld + p.i);
+  float v[16];
+  h.get(v);
+  uint4 q;
+  const int s = pack_half(v, &q);
+  if (!p.live) return;
+  store_codes(codes + p.r * c_ld + p.i, q);
+  if ((threadIdx.x & 1) == 0) scales[p.r * s_ld + p.i / kGroup] = (uint8_t)s;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack16_kernel(const Cut c, const uint8_t* codes, int64_t c_ld,
+                                                            const uint8_t* scales, int64_t s_ld, T* x, int64_t x_ld) {
+  const Place p = place_of(c);
+  if (!p.live) return;
+  float v[16];
+  unpack_half(load_codes(codes + p.r * c_ld + p.i), pow2_of(scales[p.r * s_ld + p.i / kGroup]), v);
+  store_half(x + p.r * x_ld + p.i, v);
+}
+
+// gu rows hold g then u; the packed rows 2r and 2r + 1 are row r's g and u.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) silu_mul_pack16_kernel(const Cut c, const T* gu, int64_t gu_ld, T* z,
+                                                                   int64_t z_ld, uint8_t* codes, int64_t c_ld,
+                                                                   uint8_t* scales, int64_t s_ld) {
+  const Place p = place_of(c);
+  Half<T> hg, hu;
+  hg.zero();
+  hu.zero();
+  if (p.live) {
+    hg.load(gu + p.r * gu_ld + p.i);
+    hu.load(gu + p.r * gu_ld + c.n + p.i);
+  }
+  float g[16], u[16];
+  hg.get(g);
+  hu.get(u);
+  if (p.live) {
+    float o[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) o[k] = g[k] * sigmoid32(g[k]) * u[k];
+    store_half(z + p.r * z_ld + p.i, o);
+  }
+  uint4 qg, qu;
+  const int sg = pack_half(g, &qg), su = pack_half(u, &qu);
+  if (!p.live) return;
+  store_codes(codes + 2 * p.r * c_ld + p.i, qg);
+  store_codes(codes + (2 * p.r + 1) * c_ld + p.i, qu);
+  if ((threadIdx.x & 1) == 0) {
+    scales[2 * p.r * s_ld + p.i / kGroup] = (uint8_t)sg;
+    scales[(2 * p.r + 1) * s_ld + p.i / kGroup] = (uint8_t)su;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    silu_mul_bwd16_kernel(const Cut c, const T* dz, int64_t dz_ld, const uint8_t* codes, int64_t c_ld,
+                          const uint8_t* scales, int64_t s_ld, T* dgu, int64_t dgu_ld, T* z, int64_t z_ld) {
+  const Place p = place_of(c);
+  if (!p.live) return;
+  const int64_t r2 = 2 * p.r, k0 = p.i / kGroup;
+  float d[16], g[16], u[16];
+  load_half(dz + p.r * dz_ld + p.i, d);
+  unpack_half(load_codes(codes + r2 * c_ld + p.i), pow2_of(scales[r2 * s_ld + k0]), g);
+  unpack_half(load_codes(codes + (r2 + 1) * c_ld + p.i), pow2_of(scales[(r2 + 1) * s_ld + k0]), u);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const SwigluGrad s = swiglu_grad(d[k], g[k], u[k]);
+    d[k] = s.dg;
+    g[k] = s.du;
+    u[k] = s.z;
+  }
+  store_half(dgu + p.r * dgu_ld + p.i, d);
+  store_half(dgu + p.r * dgu_ld + c.n + p.i, g);
+  if (z) store_half(z + p.r * z_ld + p.i, u);
+}
+
+// ---------------------------------------------------------------------------------------------
+// A value a lane.
+// ---------------------------------------------------------------------------------------------
+template <typename T>
+__global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, int64_t n, const T* x, int64_t x_ld,
+                                                        uint8_t* codes, int64_t c_ld, uint8_t* scales, int64_t s_ld) {
+  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
+  const int lane = threadIdx.x & 31;
+  for (int64_t g = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); g < total; g += (int64_t)gridDim.x * kWarps) {
+    const int64_t r = g / groups, i = (g - r * groups) * kGroup + lane;
+    int s;
+    const uint32_t c = pack_lane(i < n ? to_float(x[r * x_ld + i]) : 0.f, &s);
+    if (i < n) codes[r * c_ld + i] = (uint8_t)c;
+    if (lane == 0) scales[r * s_ld + i / kGroup] = (uint8_t)s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld,
+                                                          const uint8_t* scales, int64_t s_ld, T* x, int64_t x_ld) {
+  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
+  const int lane = threadIdx.x & 31;
+  for (int64_t g = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); g < total; g += (int64_t)gridDim.x * kWarps) {
+    const int64_t r = g / groups, i = (g - r * groups) * kGroup + lane;
+    if (i < n) x[r * x_ld + i] = from_float<T>(unpack_one(codes[r * c_ld + i], scales[r * s_ld + i / kGroup]));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(int64_t rows, int64_t n, const T* gu, int64_t gu_ld,
+                                                                 T* z, int64_t z_ld, uint8_t* codes, int64_t c_ld,
+                                                                 uint8_t* scales, int64_t s_ld) {
+  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
+  const int lane = threadIdx.x & 31;
+  for (int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); w < total; w += (int64_t)gridDim.x * kWarps) {
+    const int64_t r = w / groups, i = (w - r * groups) * kGroup + lane;
+    const float g = i < n ? to_float(gu[r * gu_ld + i]) : 0.f;
+    const float u = i < n ? to_float(gu[r * gu_ld + n + i]) : 0.f;
+    int sg, su;
+    const uint32_t cg = pack_lane(g, &sg), cu = pack_lane(u, &su);
+    if (i < n) {
+      z[r * z_ld + i] = from_float<T>(g * sigmoid32(g) * u);
+      codes[2 * r * c_ld + i] = (uint8_t)cg;
+      codes[(2 * r + 1) * c_ld + i] = (uint8_t)cu;
+    }
+    if (lane == 0) {
+      scales[2 * r * s_ld + i / kGroup] = (uint8_t)sg;
+      scales[(2 * r + 1) * s_ld + i / kGroup] = (uint8_t)su;
+    }
+  }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     silu_mul_bwd_kernel(int64_t rows, int64_t n, const T* dz, int64_t dz_ld, const uint8_t* codes, int64_t c_ld,
                         const uint8_t* scales, int64_t s_ld, T* dgu, int64_t dgu_ld, T* z, int64_t z_ld) {
-  const int64_t total = rows * n;
-  for (int64_t e = (int64_t)blockIdx.x * kThreads + threadIdx.x; e < total; e += (int64_t)gridDim.x * kThreads) {
-    const int64_t r = e / n, i = e - r * n, r2 = 2 * r;
+  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
+  const int lane = threadIdx.x & 31;
+  for (int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); w < total; w += (int64_t)gridDim.x * kWarps) {
+    const int64_t r = w / groups, i = (w - r * groups) * kGroup + lane, r2 = 2 * r;
+    if (i >= n) continue;
     const float g = unpack_one(codes[r2 * c_ld + i], scales[r2 * s_ld + i / kGroup]);
     const float u = unpack_one(codes[(r2 + 1) * c_ld + i], scales[(r2 + 1) * s_ld + i / kGroup]);
     const SwigluGrad d = swiglu_grad(to_float(dz[r * dz_ld + i]), g, u);
@@ -107,141 +206,22 @@ __global__ void __launch_bounds__(kThreads)
   }
 }
 
-// Sum over the CTA, the same value in every thread; ws: kWarps floats, free for the next sum on return.
-__device__ __forceinline__ float block_sum(float v, float* ws) {
-  v = warp_sum(v);
-  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float t = 0.f;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) t += ws[w];
-  __syncthreads();
-  return t;
+// One CTA per 256 halves; the sizes that a grid cannot hold (beyond 2^31 CTAs: 2^43 values) are refused.
+bool cut(int64_t rows, int64_t n, Cut* c, unsigned* grid) {
+  c->rows = rows;
+  c->n = n;
+  c->per_row = (n + kGroup - 1) / kGroup * 2;
+  c->halves = rows * c->per_row;
+  c->magic = row_magic(rows, c->per_row);
+  const int64_t blocks = (c->halves + kThreads - 1) / kThreads;
+  *grid = (unsigned)blocks;
+  return blocks <= 0x7fffffffLL;
 }
 
-struct NormFwd {
-  int64_t rows, d;
-  const void *x, *a, *w;
-  int64_t x_ld, a_ld;
-  float eps;
-  void *h, *y;
-  int64_t h_ld, y_ld;
-  uint8_t *codes, *scales;
-  int64_t c_ld, s_ld;
-  float* rstd;
-};
-
-template <typename T>
-__device__ __forceinline__ float residual(const NormFwd& a, int64_t r, int64_t i) {
-  float v = to_float(static_cast<const T*>(a.x)[r * a.x_ld + i]);
-  if (a.a) v = to_float(from_float<T>(v + to_float(static_cast<const T*>(a.a)[r * a.a_ld + i])));
-  return v;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) add_rmsnorm_pack_kernel(const NormFwd a) {
-  __shared__ float ws[kWarps];
-  const int64_t r = blockIdx.x, padded = (a.d + kGroup - 1) / kGroup * kGroup;
-  float ss = 0.f;
-  for (int64_t i = threadIdx.x; i < a.d; i += kThreads) {
-    const float v = residual<T>(a, r, i);
-    ss = fmaf(v, v, ss);
-  }
-  const float rstd = 1.0f / sqrtf(block_sum(ss, ws) / (float)a.d + a.eps);
-  if (threadIdx.x == 0) a.rstd[r] = rstd;
-  for (int64_t i = threadIdx.x; i < padded; i += kThreads) {  // whole warps: a group is a warp's 32 lanes
-    const float v = i < a.d ? residual<T>(a, r, i) : 0.f;
-    int s;
-    const uint32_t c = pack_lane(v, &s);
-    if (i < a.c_ld) a.codes[r * a.c_ld + i] = (uint8_t)c;
-    if ((threadIdx.x & 31) == 0) a.scales[r * a.s_ld + i / kGroup] = (uint8_t)s;
-    if (i < a.d) {
-      if (a.h) static_cast<T*>(a.h)[r * a.h_ld + i] = from_float<T>(v);
-      static_cast<T*>(a.y)[r * a.y_ld + i] = from_float<T>(v * rstd * to_float(static_cast<const T*>(a.w)[i]));
-    }
-  }
-}
-
-struct NormBwd {
-  int64_t rows, d;
-  const void *dy, *dh, *w;
-  int64_t dy_ld, dh_ld;
-  const uint8_t *codes, *scales;
-  int64_t c_ld, s_ld;
-  const float* rstd;
-  void *dx, *y, *dw;
-  int64_t dx_ld, y_ld;
-  float* part;  // [parts, d] partial sums of dw
-  int parts;
-};
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rmsnorm_bwd_kernel(const NormBwd a) {
-  __shared__ float ws[kWarps];
-  const int64_t r = blockIdx.x;
-  const float rstd = a.rstd[r];
-  const T *dy = static_cast<const T*>(a.dy) + r * a.dy_ld, *w = static_cast<const T*>(a.w);
-  float along = 0.f;
-  for (int64_t i = threadIdx.x; i < a.d; i += kThreads) {
-    const float xh = unpack_one(a.codes[r * a.c_ld + i], a.scales[r * a.s_ld + i / kGroup]) * rstd;
-    along = fmaf(to_float(dy[i]) * to_float(w[i]), xh, along);
-  }
-  along = block_sum(along, ws) / (float)a.d;
-  for (int64_t i = threadIdx.x; i < a.d; i += kThreads) {
-    const float xh = unpack_one(a.codes[r * a.c_ld + i], a.scales[r * a.s_ld + i / kGroup]) * rstd;
-    const float wi = to_float(w[i]);
-    float dx = rstd * (to_float(dy[i]) * wi - xh * along);
-    if (a.dh) dx += to_float(static_cast<const T*>(a.dh)[r * a.dh_ld + i]);
-    static_cast<T*>(a.dx)[r * a.dx_ld + i] = from_float<T>(dx);
-    if (a.y) static_cast<T*>(a.y)[r * a.y_ld + i] = from_float<T>(xh * wi);
-  }
-}
-
-// part[p][i] = sum of dy x^ over the p-th share of the rows.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rmsnorm_dw_part_kernel(const NormBwd a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= a.d) return;
-  const int64_t share = (a.rows + a.parts - 1) / a.parts, r0 = blockIdx.y * share, r1 = min(r0 + share, a.rows);
-  float sum = 0.f;
-  for (int64_t r = r0; r < r1; ++r) {
-    const float xh = unpack_one(a.codes[r * a.c_ld + i], a.scales[r * a.s_ld + i / kGroup]) * a.rstd[r];
-    sum = fmaf(to_float(static_cast<const T*>(a.dy)[r * a.dy_ld + i]), xh, sum);
-  }
-  a.part[blockIdx.y * a.d + i] = sum;
-}
-
-// dw = the partial sums, always added in the same order.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) rmsnorm_dw_sum_kernel(const NormBwd a) {
-  const int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (i >= a.d) return;
-  float sum = 0.f;
-  for (int p = 0; p < a.parts; ++p) sum += a.part[p * a.d + i];
-  static_cast<T*>(a.dw)[i] = from_float<T>(sum);
-}
-
-int parts_of(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>(rows / 8, 128)); }
-
-unsigned grid_of(int64_t blocks) { return (unsigned)std::max<int64_t>(1, std::min<int64_t>(blocks, 148 * 32)); }
-
-int launched() { return cudaGetLastError() == cudaSuccess ? GSA_OK : GSA_ERR_LAUNCH; }
-
-bool type_ok(int dtype) { return dtype == GSA_DTYPE_F32 || dtype == GSA_DTYPE_BF16; }
-
-// Packed rows of n values: whole 16-byte pieces of codes, a scale byte for each group.
-bool packed_ok(const uint8_t* codes, int64_t c_ld, const uint8_t* scales, int64_t s_ld, int64_t n) {
-  return codes && scales && c_ld >= (n + 15) / 16 * 16 && c_ld % 16 == 0 &&
-         reinterpret_cast<uintptr_t>(codes) % 16 == 0 && s_ld >= (n + kGroup - 1) / kGroup;
-}
-
-// Calls f with a value of the element type.
-template <typename F>
-void typed(int dtype, F f) {
-  if (dtype == GSA_DTYPE_BF16)
-    f(__nv_bfloat16());
-  else
-    f(float());
+// CTAs for the kernels of a value a lane, which stride: 32 of 8 warps for each SM.
+unsigned lane_grid(int64_t rows, int64_t n) {
+  const int64_t blocks = (rows * ((n + kGroup - 1) / kGroup) + kWarps - 1) / kWarps;
+  return (unsigned)std::min<int64_t>(blocks, 148 * 32);
 }
 
 }  // namespace
@@ -257,12 +237,17 @@ int gsa_pack_e4m3(int dtype, int64_t rows, int64_t n, const void* x, int64_t x_l
   if (rows == 0 || n == 0) return GSA_OK;
   if (!x || x_ld < 0 || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = grid_of((rows * ((n + kGroup - 1) / kGroup) + kWarps - 1) / kWarps);
   typed(dtype, [&](auto e) {
     using T = decltype(e);
-    pack_kernel<T><<<grid, kThreads, 0, s>>>(rows, n, static_cast<const T*>(x), x_ld, codes, c_ld, scales, s_ld);
+    const T* in = static_cast<const T*>(x);
+    Cut c;
+    unsigned grid;
+    if (n % 16 == 0 && halves_ok<T>(x, x_ld) && cut(rows, n, &c, &grid))
+      pack16_kernel<T><<<grid, kThreads, 0, s>>>(c, in, x_ld, codes, c_ld, scales, s_ld);
+    else
+      pack_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, x_ld, codes, c_ld, scales, s_ld);
   });
-  return launched();
+  return launch_status();
 }
 
 int gsa_unpack_e4m3(int dtype, int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld, const uint8_t* scales,
@@ -271,12 +256,17 @@ int gsa_unpack_e4m3(int dtype, int64_t rows, int64_t n, const uint8_t* codes, in
   if (rows == 0 || n == 0) return GSA_OK;
   if (!x || x_ld < n || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = grid_of((rows * n + kThreads - 1) / kThreads);
   typed(dtype, [&](auto e) {
     using T = decltype(e);
-    unpack_kernel<T><<<grid, kThreads, 0, s>>>(rows, n, codes, c_ld, scales, s_ld, static_cast<T*>(x), x_ld);
+    T* out = static_cast<T*>(x);
+    Cut c;
+    unsigned grid;
+    if (n % 16 == 0 && halves_ok<T>(x, x_ld) && cut(rows, n, &c, &grid))
+      unpack16_kernel<T><<<grid, kThreads, 0, s>>>(c, codes, c_ld, scales, s_ld, out, x_ld);
+    else
+      unpack_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, codes, c_ld, scales, s_ld, out, x_ld);
   });
-  return launched();
+  return launch_status();
 }
 
 int gsa_silu_mul_pack(int dtype, int64_t rows, int64_t n, const void* gu, int64_t gu_ld, void* z, int64_t z_ld,
@@ -285,13 +275,19 @@ int gsa_silu_mul_pack(int dtype, int64_t rows, int64_t n, const void* gu, int64_
   if (rows == 0 || n == 0) return GSA_OK;
   if (!gu || gu_ld < 0 || !z || z_ld < n || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = grid_of((rows * ((n + kGroup - 1) / kGroup) + kWarps - 1) / kWarps);
   typed(dtype, [&](auto e) {
     using T = decltype(e);
-    silu_mul_pack_kernel<T><<<grid, kThreads, 0, s>>>(rows, n, static_cast<const T*>(gu), gu_ld, static_cast<T*>(z),
-                                                      z_ld, codes, c_ld, scales, s_ld);
+    const T* in = static_cast<const T*>(gu);
+    T* out = static_cast<T*>(z);
+    Cut c;
+    unsigned grid;
+    if (n % 16 == 0 && halves_ok<T>(gu, gu_ld) && halves_ok<T>(z, z_ld) && cut(rows, n, &c, &grid))
+      silu_mul_pack16_kernel<T><<<grid, kThreads, 0, s>>>(c, in, gu_ld, out, z_ld, codes, c_ld, scales, s_ld);
+    else
+      silu_mul_pack_kernel<T>
+          <<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, gu_ld, out, z_ld, codes, c_ld, scales, s_ld);
   });
-  return launched();
+  return launch_status();
 }
 
 int gsa_silu_mul_packed_backward(int dtype, int64_t rows, int64_t n, const void* dz, int64_t dz_ld,
@@ -302,59 +298,21 @@ int gsa_silu_mul_packed_backward(int dtype, int64_t rows, int64_t n, const void*
   if (!dz || dz_ld < 0 || !dgu || dgu_ld < 2 * n || (z && z_ld < n) || !packed_ok(codes, c_ld, scales, s_ld, n))
     return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = grid_of((rows * n + kThreads - 1) / kThreads);
   typed(dtype, [&](auto e) {
     using T = decltype(e);
-    silu_mul_bwd_kernel<T><<<grid, kThreads, 0, s>>>(rows, n, static_cast<const T*>(dz), dz_ld, codes, c_ld, scales,
-                                                     s_ld, static_cast<T*>(dgu), dgu_ld, static_cast<T*>(z), z_ld);
+    const T* in = static_cast<const T*>(dz);
+    T *out = static_cast<T*>(dgu), *again = static_cast<T*>(z);
+    Cut c;
+    unsigned grid;
+    if (n % 16 == 0 && halves_ok<T>(dz, dz_ld) && halves_ok<T>(dgu, dgu_ld) && (!z || halves_ok<T>(z, z_ld)) &&
+        cut(rows, n, &c, &grid))
+      silu_mul_bwd16_kernel<T>
+          <<<grid, kThreads, 0, s>>>(c, in, dz_ld, codes, c_ld, scales, s_ld, out, dgu_ld, again, z_ld);
+    else
+      silu_mul_bwd_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, dz_ld, codes, c_ld, scales, s_ld,
+                                                                     out, dgu_ld, again, z_ld);
   });
-  return launched();
-}
-
-int gsa_add_rmsnorm_pack(int dtype, int64_t rows, int64_t d, const void* x, int64_t x_ld, const void* a, int64_t a_ld,
-                         const void* weight, float eps, void* h, int64_t h_ld, void* y, int64_t y_ld, uint8_t* codes,
-                         int64_t c_ld, uint8_t* scales, int64_t s_ld, float* rstd, gsa_stream_t stream) {
-  if (!type_ok(dtype) || rows < 0 || d < 1 || rows > 0x7fffffffLL) return GSA_ERR_BAD_ARG;
-  if (rows == 0) return GSA_OK;
-  if (!x || x_ld < 0 || (a && a_ld < 0) || !weight || !y || y_ld < d || (h && (!a || h_ld < d)) || !rstd ||
-      !packed_ok(codes, c_ld, scales, s_ld, d))
-    return GSA_ERR_BAD_ARG;
-  const NormFwd p{rows, d, x, a, weight, x_ld, a_ld, eps, h, y, h_ld, y_ld, codes, scales, c_ld, s_ld, rstd};
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  typed(dtype, [&](auto e) { add_rmsnorm_pack_kernel<decltype(e)><<<(unsigned)rows, kThreads, 0, s>>>(p); });
-  return launched();
-}
-
-int64_t gsa_rmsnorm_packed_workspace_size(int64_t rows, int64_t d) {
-  return rows > 0 && d > 0 ? parts_of(rows) * d * (int64_t)sizeof(float) : 0;
-}
-
-int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* dy, int64_t dy_ld, const void* dh,
-                                int64_t dh_ld, const void* weight, const uint8_t* codes, int64_t c_ld,
-                                const uint8_t* scales, int64_t s_ld, const float* rstd, void* dx, int64_t dx_ld,
-                                void* y, int64_t y_ld, void* dw, void* workspace, int64_t workspace_bytes,
-                                gsa_stream_t stream) {
-  if (!type_ok(dtype) || rows < 0 || d < 1 || rows > 0x7fffffffLL) return GSA_ERR_BAD_ARG;
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (rows == 0) {
-    if (!dw) return GSA_OK;
-    return cudaMemsetAsync(dw, 0, d * (dtype == GSA_DTYPE_BF16 ? 2 : 4), s) == cudaSuccess ? GSA_OK : GSA_ERR_CUDA;
-  }
-  if (!dy || dy_ld < 0 || (dh && dh_ld < 0) || !weight || !rstd || !dx || dx_ld < d || (y && y_ld < d) ||
-      !packed_ok(codes, c_ld, scales, s_ld, d))
-    return GSA_ERR_BAD_ARG;
-  if (dw && (!workspace || workspace_bytes < gsa_rmsnorm_packed_workspace_size(rows, d))) return GSA_ERR_WORKSPACE;
-  const NormBwd p{rows, d,    dy,   dh, weight, dy_ld, dh_ld, codes, scales, c_ld,
-                  s_ld, rstd, dx,   y,  dw,     dx_ld, y_ld,  static_cast<float*>(workspace), parts_of(rows)};
-  typed(dtype, [&](auto e) {
-    using T = decltype(e);
-    rmsnorm_bwd_kernel<T><<<(unsigned)rows, kThreads, 0, s>>>(p);
-    if (!dw) return;
-    const unsigned cols = (unsigned)((d + kThreads - 1) / kThreads);
-    rmsnorm_dw_part_kernel<T><<<dim3(cols, p.parts), kThreads, 0, s>>>(p);
-    rmsnorm_dw_sum_kernel<T><<<cols, kThreads, 0, s>>>(p);
-  });
-  return launched();
+  return launch_status();
 }
 
 }  // extern "C"

@@ -45,4 +45,197 @@ __device__ __forceinline__ uint32_t finite_abs_bits(float x) {
 }
 __device__ __forceinline__ float inf_to_nan(float x) { return isinf(x) ? __int_as_float(0x7fc00000) : x; }
 
+// One value a lane: a warp's 32 are a group.  Returns the code (in the low byte).
+__device__ __forceinline__ uint32_t pack_lane(float x, int* scale) {
+  const int s = scale_byte(__reduce_max_sync(0xffffffffu, finite_abs_bits(x)));
+  *scale = s;
+  return to_e4m3x2(inf_to_nan(x) * inv_pow2_of(s), 0.f) & 0xffu;
+}
+__device__ __forceinline__ float unpack_one(uint8_t code, uint8_t scale) {
+  return from_e4m3x2(code).x * pow2_of(scale);
+}
+
+// ---------------------------------------------------------------------------------------------
+// 16 values a thread: half a group.  Their loads and stores are 32-byte ones (a whole sector a thread), kept out
+// of L1, where nothing reads them twice.
+// ---------------------------------------------------------------------------------------------
+struct Words8 {
+  uint32_t w[8];
+};
+__device__ __forceinline__ Words8 load32(const void* p) {
+  Words8 r;
+  asm("ld.global.nc.L1::no_allocate.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+      : "l"(p));
+  return r;
+}
+// The same through L1, for what neighbouring CTAs read again.
+__device__ __forceinline__ Words8 load32_shared(const void* p) {
+  Words8 r;
+  asm("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+      : "=r"(r.w[0]), "=r"(r.w[1]), "=r"(r.w[2]), "=r"(r.w[3]), "=r"(r.w[4]), "=r"(r.w[5]), "=r"(r.w[6]), "=r"(r.w[7])
+      : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void store32(void* p, const Words8& r) {
+  asm volatile("st.global.L1::no_allocate.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r.w[0]),
+               "r"(r.w[1]), "r"(r.w[2]), "r"(r.w[3]), "r"(r.w[4]), "r"(r.w[5]), "r"(r.w[6]), "r"(r.w[7])
+               : "memory");
+}
+
+// 16 values in their type, and their conversions.
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  Words8 a;
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { a = load32(p); }
+  __device__ __forceinline__ void load_shared(const __nv_bfloat16* p) { a = load32_shared(p); }
+  __device__ __forceinline__ void zero() { a = Words8{}; }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[2 * i] = __uint_as_float(a.w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(a.w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+      a.w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* p) const { store32(p, a); }
+};
+template <>
+struct Half<float> {
+  Words8 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = load32(p);
+    b = load32(p + 8);
+  }
+  __device__ __forceinline__ void load_shared(const float* p) {
+    a = load32_shared(p);
+    b = load32_shared(p + 8);
+  }
+  __device__ __forceinline__ void zero() { a = b = Words8{}; }
+  __device__ __forceinline__ void get(float* v) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = __uint_as_float(a.w[i]);
+      v[8 + i] = __uint_as_float(b.w[i]);
+    }
+  }
+  __device__ __forceinline__ void set(const float* v) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      a.w[i] = __float_as_uint(v[i]);
+      b.w[i] = __float_as_uint(v[8 + i]);
+    }
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    store32(p, a);
+    store32(p + 8, b);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void load_half(const T* p, float* v) {
+  Half<T> h;
+  h.load(p);
+  h.get(v);
+}
+template <typename T>
+__device__ __forceinline__ void store_half(T* p, const float* v) {
+  Half<T> h;
+  h.set(v);
+  h.store(p);
+}
+
+// A group held by two neighbouring lanes (every lane of the warp calls this): the scale byte, and this lane's 16
+// codes.  Lanes without values pass zeros.
+__device__ __forceinline__ int pack_half(float* v, uint4* codes) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  if (m >= 0x7f800000u) {  // rare: the scale goes by the finite values, infinities convert as NaN
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      m = max(m, finite_abs_bits(v[i]));
+      v[i] = inf_to_nan(v[i]);
+    }
+  }
+  m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const int s = scale_byte(m);
+  const float f = inv_pow2_of(s);
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = to_e4m3x2(v[4 * i] * f, v[4 * i + 1] * f) |
+           (uint32_t)to_e4m3x2(v[4 * i + 2] * f, v[4 * i + 3] * f) << 16;
+  *codes = make_uint4(w[0], w[1], w[2], w[3]);
+  return s;
+}
+
+__device__ __forceinline__ void unpack_half(const uint4& codes, float scale, float* v) {
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 lo = from_e4m3x2((uint16_t)w[i]), hi = from_e4m3x2((uint16_t)(w[i] >> 16));
+    v[4 * i] = lo.x * scale;
+    v[4 * i + 1] = lo.y * scale;
+    v[4 * i + 2] = hi.x * scale;
+    v[4 * i + 3] = hi.y * scale;
+  }
+}
+
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p) {
+  uint4 r;
+  asm("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+      : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+      : "l"(p));
+  return r;
+}
+__device__ __forceinline__ void store_codes(uint8_t* p, const uint4& c) {
+  asm volatile("st.global.L1::no_allocate.v4.b32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(c.x), "r"(c.y), "r"(c.z),
+               "r"(c.w)
+               : "memory");
+}
+
+// floor(n / d) for n d < 2^64, d > 1, with m = ceil(2^64 / d); d = 1 (a single row) is passed as m = 0 and gives 0
+// for n < d of the one row.
+__device__ __forceinline__ int64_t row_of(int64_t n, uint64_t m) { return (int64_t)__umul64hi((uint64_t)n, m); }
+inline uint64_t row_magic(int64_t rows, int64_t d) { return rows == 1 ? 0 : ~0ull / (uint64_t)d + 1; }
+
+inline bool type_ok(int dtype) { return dtype == GSA_DTYPE_F32 || dtype == GSA_DTYPE_BF16; }
+
+// Packed rows of n values: whole 16-byte pieces of codes, a scale byte for each group.
+inline bool packed_ok(const uint8_t* codes, int64_t c_ld, const uint8_t* scales, int64_t s_ld, int64_t n) {
+  return codes && scales && c_ld >= (n + 15) / 16 * 16 && c_ld % 16 == 0 &&
+         reinterpret_cast<uintptr_t>(codes) % 16 == 0 && s_ld >= (n + kGroup - 1) / kGroup;
+}
+
+// Calls f with a value of the element type.
+template <typename F>
+inline void typed(int dtype, F f) {
+  if (dtype == GSA_DTYPE_BF16)
+    f(__nv_bfloat16());
+  else
+    f(float());
+}
+
+inline int launch_status() { return cudaGetLastError() == cudaSuccess ? GSA_OK : GSA_ERR_LAUNCH; }
+
+// Whether rows of a tensor can be read or written 16 values at a time.
+template <typename T>
+inline bool halves_ok(const void* p, int64_t ld) {
+  return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld % 16 == 0;
+}
+template <>
+inline bool halves_ok<float>(const void* p, int64_t ld) {
+  return reinterpret_cast<uintptr_t>(p) % 32 == 0 && ld % 8 == 0;
+}
+
 }  // namespace gsa
