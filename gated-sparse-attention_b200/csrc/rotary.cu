@@ -8,6 +8,10 @@
 // angle (p f of 2^20 radians in 32 bits is off by 2^-4); sine and cosine of the fraction are 32-bit.  A CTA takes
 // a few tokens, evaluates each token's rd/2 angles once into shared memory (all its heads share them) and
 // then streams the tokens' heads.  Bound by the bytes of q and k, read once and written once.
+//
+// A thread owns one place of a token -- a head and V neighbouring pairs of it (or 2 V pass-through values) -- and
+// walks the CTA's tokens with it, four in flight, so the place is worked out once.  V values are one
+// load: 16 bytes where rd, D, the strides and the addresses are multiples of that, else 2 values, else 1.
 #include <algorithm>
 
 #include "kernels.cuh"
@@ -15,8 +19,9 @@
 namespace gsa {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxTokens = 16;
+constexpr int kMaxThreads = 512;
+constexpr int kMaxTokens = 8;
+constexpr int kFlight = 4;        // tokens whose loads are in flight
 constexpr int kMaxAngles = 4096;  // (token, pair) entries of the shared table: 32 KB
 
 struct Side {  // q or k: strides in elements
@@ -40,13 +45,9 @@ struct RotaryArgs {
   float factor;
   int inverse;
   int tokens;  // per CTA
-  int units;   // of a head: pairs, then pass-through values
-  uint32_t m_units, m_heads;
+  int turn_units, units;  // of a head: units that turn, all
   int* err;
 };
-
-// n / d for n * d < 2^32 with m = ceil(2^32 / d); d = 1 has no 32-bit m and is passed as m = 0.
-__device__ __forceinline__ uint32_t fast_div(uint32_t n, uint32_t m) { return m ? __umulhi(n, m) : n; }
 
 // (c, s) of one token's pair i.
 __device__ __forceinline__ float2 angle_of(const RotaryArgs& a, int64_t p, int i) {
@@ -71,9 +72,100 @@ __device__ __forceinline__ float2 angle_of(const RotaryArgs& a, int64_t p, int i
 __device__ __forceinline__ float turn0(float x0, float x1, float2 cs) { return fadd(fmul(x0, cs.x), -fmul(x1, cs.y)); }
 __device__ __forceinline__ float turn1(float x0, float x1, float2 cs) { return fadd(fmul(x1, cs.x), fmul(x0, cs.y)); }
 
-template <typename T, bool kInterleaved>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
-  extern __shared__ float2 angles[];
+// V values as one load or store.
+template <int kBytes>
+struct Raw;
+template <>
+struct Raw<16> {
+  using type = uint4;
+};
+template <>
+struct Raw<8> {
+  using type = uint2;
+};
+template <>
+struct Raw<4> {
+  using type = uint32_t;
+};
+template <>
+struct Raw<2> {
+  using type = uint16_t;
+};
+template <typename T, int V>
+union Vec {
+  typename Raw<sizeof(T) * V>::type raw;
+  T v[V];
+  __device__ __forceinline__ Vec() : raw{} {}
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const decltype(raw)*>(p); }
+  __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<decltype(raw)*>(p) = raw; }
+};
+
+// One place of a token: where its two vectors are, relative to the token's head 0.
+struct Place {
+  int64_t in, out;  // of the head
+  int i0, i1;       // the vectors' first values; i1 < 0: the second is not there
+  int angle;        // of the unit's first pair; < 0: passes through
+  bool is_k;
+};
+
+template <typename T, int V, bool kInterleaved>
+__device__ __forceinline__ Place place_of(const RotaryArgs& a, int item) {
+  const int h = item / a.units, u = item - h * a.units, half = a.rd / 2;
+  Place p;
+  p.is_k = h >= a.q.heads;
+  const Side& s = p.is_k ? a.k : a.q;
+  const int hh = p.is_k ? h - a.q.heads : h;
+  p.in = hh * s.ih;
+  p.out = hh * s.oh;
+  if (u < a.turn_units) {
+    p.i0 = kInterleaved ? 2 * u * V : u * V;
+    p.i1 = kInterleaved ? p.i0 + V : p.i0 + half;
+    p.angle = u * V;
+  } else {
+    p.i0 = a.rd + (u - a.turn_units) * 2 * V;
+    p.i1 = p.i0 + V < a.D ? p.i0 + V : -1;
+    p.angle = -1;
+  }
+  return p;
+}
+
+// x0, x1: the unit's two vectors, turned in place.  cs: the unit's V angles.
+template <typename T, int V, bool kInterleaved>
+__device__ __forceinline__ void turn(Vec<T, V>& x0, Vec<T, V>& x1, const float2* cs) {
+  if (kInterleaved) {
+    // values 2j, 2j + 1 of the 2 V are pair j
+    T w[2 * V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      w[j] = x0.v[j];
+      w[V + j] = x1.v[j];
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 c = cs[j];
+      const float a = to_float(w[2 * j]), b = to_float(w[2 * j + 1]);
+      w[2 * j] = from_float<T>(turn0(a, b, c));
+      w[2 * j + 1] = from_float<T>(turn1(a, b, c));
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      x0.v[j] = w[j];
+      x1.v[j] = w[V + j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float2 c = cs[j];
+      const float a = to_float(x0.v[j]), b = to_float(x1.v[j]);
+      x0.v[j] = from_float<T>(turn0(a, b, c));
+      x1.v[j] = from_float<T>(turn1(a, b, c));
+    }
+  }
+}
+
+template <typename T, int V, bool kInterleaved>
+__global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a) {
+  extern __shared__ __align__(16) float2 angles[];
   __shared__ int64_t base[kMaxTokens][4];  // element offsets of the token: q in, q out, k in, k out
   const int half = a.rd / 2;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
@@ -85,30 +177,38 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     base[threadIdx.x][2] = b * a.k.ib + l * a.k.il;
     base[threadIdx.x][3] = b * a.k.ob + l * a.k.ol;
   }
-  for (int e = threadIdx.x; e < n_tok * half; e += kThreads) {
-    const int64_t t = t0 + e / half, b = t / a.L, l = t - b * a.L;
-    angles[e] = angle_of(a, a.pos[b * a.pb + l * a.pl], e % half);
+  for (int e = threadIdx.x; e < n_tok * half; e += blockDim.x) {
+    const int tok = e / half;
+    const int64_t t = t0 + tok, b = t / a.L, l = t - b * a.L;
+    angles[e] = angle_of(a, a.pos[b * a.pb + l * a.pl], e - tok * half);
   }
   __syncthreads();
-  const int heads = a.q.heads + a.k.heads;
-  const uint32_t items = (uint32_t)n_tok * heads * a.units;
-  for (uint32_t it = threadIdx.x; it < items; it += kThreads) {
-    const uint32_t row = fast_div(it, a.m_units), u = it - row * a.units;
-    const uint32_t tok = fast_div(row, a.m_heads), h = row - tok * heads;
-    const bool is_k = (int)h >= a.q.heads;
-    const Side& s = is_k ? a.k : a.q;
-    const int hh = is_k ? h - a.q.heads : h;
-    const T* in = static_cast<const T*>(s.in) + base[tok][is_k ? 2 : 0] + hh * s.ih;
-    T* out = static_cast<T*>(s.out) + base[tok][is_k ? 3 : 1] + hh * s.oh;
-    if ((int)u < half) {
-      const int i0 = kInterleaved ? 2 * u : u, i1 = kInterleaved ? 2 * u + 1 : u + half;
-      const float2 cs = angles[tok * half + u];
-      const float x0 = to_float(in[i0]), x1 = to_float(in[i1]);
-      out[i0] = from_float<T>(turn0(x0, x1, cs));
-      out[i1] = from_float<T>(turn1(x0, x1, cs));
-    } else {
-      const int i = a.rd + (u - half);
-      out[i] = in[i];
+  const int items = (a.q.heads + a.k.heads) * a.units;
+  for (int item = threadIdx.x; item < items; item += blockDim.x) {
+    const Place p = place_of<T, V, kInterleaved>(a, item);
+    const Side& s = p.is_k ? a.k : a.q;
+    const T* in = static_cast<const T*>(s.in) + p.in;
+    T* out = static_cast<T*>(s.out) + p.out;
+    const int64_t* at = &base[0][p.is_k ? 2 : 0];
+    if (p.angle < 0 && in == out) continue;  // rotated in place: the rest is where it belongs
+    // four tokens' loads before the first store, which may be to the same tensor
+    for (int tok0 = 0; tok0 < n_tok; tok0 += kFlight) {
+      Vec<T, V> x0[kFlight], x1[kFlight];
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        if (tok0 + j >= n_tok) break;
+        const T* x = in + at[4 * (tok0 + j)];
+        x0[j].load(x + p.i0);
+        if (p.i1 >= 0) x1[j].load(x + p.i1);
+      }
+#pragma unroll
+      for (int j = 0; j < kFlight; ++j) {
+        if (tok0 + j >= n_tok) break;
+        T* y = out + at[4 * (tok0 + j) + 1];
+        if (p.angle >= 0) turn<T, V, kInterleaved>(x0[j], x1[j], &angles[(tok0 + j) * half + p.angle]);
+        x0[j].store(y + p.i0);
+        if (p.i1 >= 0) x1[j].store(y + p.i1);
+      }
     }
   }
 }
@@ -123,18 +223,45 @@ Side side_of(const gsa_rotary_side* s) {
   return Side{s->in, s->out, s->heads, s->in_b, s->in_l, s->in_h, s->out_b, s->out_l, s->out_h};
 }
 
-uint32_t magic(uint32_t d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
+bool vec_ok(const Side& s, int64_t V, int64_t esz) {
+  const int64_t all = s.ib | s.il | s.ih | s.ob | s.ol | s.oh;
+  return all % V == 0 && (reinterpret_cast<uintptr_t>(s.in) | reinterpret_cast<uintptr_t>(s.out)) % (V * esz) == 0;
+}
 
-template <typename T>
-int launch_typed(const RotaryArgs& a, int interleaved, cudaStream_t stream) {
-  const int64_t T_all = a.B * a.L, grid = (T_all + a.tokens - 1) / a.tokens;
+// Whether vectors of V values tile the heads: whole vectors of the turned part (of each of its halves), and of the
+// rest.
+bool tiles(const RotaryArgs& a, int interleaved, int64_t V, int64_t esz) {
+  return (interleaved ? a.rd % (2 * V) : a.rd / 2 % V) == 0 && a.D % V == 0 && vec_ok(a.q, V, esz) &&
+         (a.k.heads == 0 || vec_ok(a.k, V, esz));
+}
+
+template <typename T, int V>
+int launch_vec(RotaryArgs a, int interleaved, cudaStream_t stream) {
+  a.turn_units = a.rd / 2 / V;
+  a.units = a.turn_units + (a.D - a.rd + 2 * V - 1) / (2 * V);
+  const int items = (a.q.heads + a.k.heads) * a.units;
+  // threads: all places of a token in as few even rounds as fit
+  const int rounds = (items + kMaxThreads - 1) / kMaxThreads;
+  const int threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;
+  // tokens a CTA: up to kMaxTokens, which spreads the angles' cost, once that leaves four CTAs for each SM
+  const int64_t n = a.B * a.L;
+  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(+kMaxTokens, kMaxAngles / (a.rd / 2)), n / (4 * 148)));
+  const int64_t grid = (n + a.tokens - 1) / a.tokens;
   if (grid > 0x7fffffffLL) return GSA_ERR_BAD_ARG;
   const size_t smem = (size_t)a.tokens * (a.rd / 2) * sizeof(float2);
   if (interleaved)
-    rotary_kernel<T, true><<<(unsigned)grid, kThreads, smem, stream>>>(a);
+    rotary_kernel<T, V, true><<<(unsigned)grid, threads, smem, stream>>>(a);
   else
-    rotary_kernel<T, false><<<(unsigned)grid, kThreads, smem, stream>>>(a);
+    rotary_kernel<T, V, false><<<(unsigned)grid, threads, smem, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? GSA_OK : GSA_ERR_LAUNCH;
+}
+
+template <typename T>
+int launch_typed(const RotaryArgs& a, int interleaved, cudaStream_t stream) {
+  constexpr int kWide = 16 / sizeof(T);
+  if (tiles(a, interleaved, kWide, sizeof(T))) return launch_vec<T, kWide>(a, interleaved, stream);
+  if (tiles(a, interleaved, 2, sizeof(T))) return launch_vec<T, 2>(a, interleaved, stream);
+  return launch_vec<T, 1>(a, interleaved, stream);
 }
 
 }  // namespace
@@ -176,12 +303,6 @@ extern "C" int gsa_rotary(int dtype, int64_t B, int64_t L, int32_t D, int32_t rd
   a.inverse = inverse;
   int st = device_error_word(&a.err);
   if (st) return st;
-  const int heads = a.q.heads + a.k.heads;
-  a.units = rd / 2 + (D - rd);
-  const int per_token = heads * a.units;
-  a.tokens = std::max(1, std::min(std::min((int)kMaxTokens, kMaxAngles / (rd / 2)), (4 * kThreads + per_token - 1) / per_token));
-  a.m_units = magic(a.units);
-  a.m_heads = magic(heads);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == GSA_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(a, interleaved, s)
                                  : launch_typed<float>(a, interleaved, s);
