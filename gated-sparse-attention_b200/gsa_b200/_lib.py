@@ -113,13 +113,14 @@ SIGNATURES = {
     "gsa_add_rmsnorm_pack": [INT, I64, I64, P, I64, P, I64, P, F32, P, I64, P, I64, P, I64, P, I64, P, P],
     "gsa_rmsnorm_packed_workspace_size": [I64, I64],
     "gsa_rmsnorm_packed_backward": [INT, I64, I64, P, I64, P, I64, P, P, I64, P, I64, P, P, I64, P, I64, P, P, I64, P],
-    "gsa_next_token_loss": [INT, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, P, P, I64, I64, P],
+    "gsa_next_token_loss": [INT, I64, I64, I64, P, I64, I64, P, I64, I64, I64, P, P, I64, I64, P, I64, P],
+    "gsa_next_token_loss_workspace_size": [],
     "gsa_scale": [INT, I64, P, P, P],
 }
 _RESTYPES = {"gsa_version": C.c_char_p, "gsa_workspace_size": C.c_int64,
              "gsa_survivors_workspace_size": C.c_int64, "gsa_sdpa_workspace_size": C.c_int64,
              "gsa_survivors_fused_workspace_size": C.c_int64,
-             "gsa_rmsnorm_packed_workspace_size": C.c_int64,
+             "gsa_rmsnorm_packed_workspace_size": C.c_int64, "gsa_next_token_loss_workspace_size": C.c_int64,
              "gsa_decode_workspace_size": C.c_int64, "gsa_proj_fused_rows": C.c_int64}
 
 _lib = None

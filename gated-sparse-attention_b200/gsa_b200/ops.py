@@ -914,10 +914,12 @@ def next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: in
     B, L, V = logits.shape
     x = logits if V == 1 or logits.stride(2) == 1 else logits.contiguous()
     loss = torch.empty((), device=logits.device, dtype=torch.float32)
-    rows = torch.empty(B * L, device=logits.device, dtype=torch.float32)
+    nbytes = _lib.lib().gsa_next_token_loss_workspace_size()
+    ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
     grad = torch.empty(B, L, V, device=logits.device, dtype=logits.dtype) if want_grad else None
     _run(logits, "gsa_next_token_loss", code, B, L, V, x.data_ptr(), x.stride(0), x.stride(1), labels.data_ptr(),
-         labels.stride(0), labels.stride(1), int(ignore_index), rows.data_ptr(), loss.data_ptr(), _ptr(grad), L * V, V)
+         labels.stride(0), labels.stride(1), int(ignore_index), loss.data_ptr(), _ptr(grad), L * V, V,
+         ws.data_ptr(), nbytes)
     return loss, grad
 
 

@@ -400,14 +400,15 @@ int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* 
  * logits [B, L, V] predicts labels[b, t + 1]; the last position, and labels equal to ignore_index, do not count.
  *   loss [1] fp32 = mean over the counted positions of (log sum exp(x) - x[label]); NaN if none counts
  *   grad (nullable) [B, L, V] dtype = (softmax(x) - onehot(label)) / count; 0 in positions that do not count
- *   row_loss [B * L] fp32: each position's loss (0 where it does not count)
- * Logits of -inf have probability 0.  A counted label outside [0, V) gives NaN and GSA_ERR_INDEX.
+ *   workspace  gsa_next_token_loss_workspace_size() bytes (the same for every size), 16-byte aligned
+ * V <= 2^30.  Logits of -inf have probability 0.  A counted label outside [0, V) gives NaN and GSA_ERR_INDEX.
  * gsa_scale: x[0 .. n) *= *factor (a device scalar; 1 leaves x unread).
  */
 int gsa_next_token_loss(int dtype, int64_t B, int64_t L, int64_t V, const void* logits, int64_t x_bstride,
                         int64_t x_lstride, const int64_t* labels, int64_t lab_bstride, int64_t lab_lstride,
-                        int64_t ignore_index, float* row_loss, float* loss, void* grad, int64_t g_bstride,
-                        int64_t g_lstride, gsa_stream_t stream);
+                        int64_t ignore_index, float* loss, void* grad, int64_t g_bstride, int64_t g_lstride,
+                        void* workspace, int64_t workspace_bytes, gsa_stream_t stream);
+int64_t gsa_next_token_loss_workspace_size(void);
 int gsa_scale(int dtype, int64_t n, void* x, const float* factor, gsa_stream_t stream);
 
 /*

@@ -152,10 +152,12 @@ def test_loss_entry_points_refuse():
 
     lib, p = _lib.lib(), _p()
 
-    def call(dtype=1, B=2, L=4, V=10, x=p, labels=p, rows=p, loss=p, grad=p, g_b=40, g_l=10):
-        return lib.gsa_next_token_loss(dtype, B, L, V, x, 40, 10, labels, 4, 1, -100, rows, loss, grad, g_b, g_l, None)
+    def call(dtype=1, B=2, L=4, V=10, x=p, labels=p, loss=p, grad=p, g_b=40, g_l=10, ws=p, nbytes=1 << 20):
+        return lib.gsa_next_token_loss(dtype, B, L, V, x, 40, 10, labels, 4, 1, -100, loss, grad, g_b, g_l, ws, nbytes, None)
 
     assert call(dtype=9) == 1 and call(B=-1) == 1 and call(V=0) == 1 and call(x=None) == 1 and call(labels=None) == 1
-    assert call(rows=None) == 1 and call(loss=None) == 1 and call(g_l=9) == 1 and call(g_b=9) == 1
+    assert call(loss=None) == 1 and call(g_l=9) == 1 and call(g_b=9) == 1
+    assert call(ws=None) == 3 and call(nbytes=lib.gsa_next_token_loss_workspace_size() - 1) == 3
+    assert call(ws=C.c_void_p(264)) == 3
     assert lib.gsa_scale(1, -1, p, p, None) == 1 and lib.gsa_scale(1, 4, None, p, None) == 1
     assert lib.gsa_scale(4, 4, p, p, None) == 1 and lib.gsa_scale(1, 0, None, None, None) == 0
