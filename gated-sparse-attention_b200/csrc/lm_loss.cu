@@ -4,14 +4,14 @@
 //   loss = mean over the counted positions of (log sum_v e^{x_v} - x_target)
 //   grad = (softmax(x) - onehot(target)) / count, zero in the rows that do not count
 //
-// A CTA takes a row (a warp takes one of up to kWarpRow values): its maximum and sum in one pass (online), then the
-// gradient from a second reading, which the L2 serves -- the rows in flight, 2 for each SM, are 76 MB of 128,256
-// bf16 logits.  So HBM sees each logit once and each gradient value once, which bounds it.
-//
-// Exponentials are 2^((x - m) log2 e) with the difference first: rows masked with the type's lowest value keep
-// their weights, which x log2 e - m log2 e would lose to overflow.  Sums are in 32 bits within a row and in 64
-// across rows; each CTA adds its rows in order and one CTA adds the CTAs' sums in order, so a loss is the same bits
-// every time.
+// A CTA takes a row (a warp takes one of up to 4 KB): its maximum and sum in one pass (online), then the gradient
+// from a second reading, which registers serve for short rows and the L2 for long ones: the rows in flight are up to
+// 76 MB.  So HBM sees each logit about once (1.1 times for rows of 250 KB) and each gradient value once.
+// Exponentials are 2^(x log2 e - M) by one multiply-add (two values an instruction) and one ex2, M the rounded m log2 e:
+// M is what the sums and the gradient share, so its rounding cancels.  Values under kLow, where that would overflow,
+// weigh 0 beside any other; a row that has nothing else (masked throughout with the type's lowest value, or with
+// -inf) is taken by differences first.  Sums are in 32 bits within a row and in 64 across rows; each CTA adds its
+// rows in order and one CTA adds the CTAs' sums in order, so a loss is the same bits every time.
 #include <algorithm>
 
 #include "kernels.cuh"
@@ -21,13 +21,12 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
-constexpr int kPerSm = 2;
-constexpr int kMaxGrid = 148 * 4;
+constexpr int kMaxGrid = 148 * 16;
 constexpr int kCounters = 64;         // CTAs of the count kernel
-constexpr int64_t kSelfCount = 16384;  // labels up to which every CTA counts for itself
-constexpr int kWarpRow = 2048;
+constexpr int64_t kSelfCount = 2048;  // labels up to which every CTA counts for itself
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLn2 = 0.693147181f;
+constexpr float kLow = -1e38f;
 
 struct Workspace {
   double sums[kMaxGrid];      // of each CTA's rows
@@ -47,8 +46,24 @@ struct LossArgs {
   int64_t gb, gl;
   float* loss;
   int* err;
-  int counted;  // ws->counts holds the count
+  int counted;     // ws->counts holds the count
+  uint64_t magic;  // ceil(2^64 / L), 0 for L = 1
 };
+
+struct Position {
+  int64_t b, t;
+};
+// Sequence and token of row r < B L: by one multiplication, exact for r L < 2^64.
+__device__ __forceinline__ Position position_of(const LossArgs& a, int64_t r) {
+  const int64_t b = a.magic ? (int64_t)__umul64hi((uint64_t)r, a.magic) : r;
+  return {b, r - b * a.L};
+}
+// What row r predicts: its label, or ignore_index past the end and for a sequence's last row.
+__device__ __forceinline__ int64_t target_of(const LossArgs& a, int64_t r) {
+  if (r >= a.B * a.L) return a.ignore;
+  const Position p = position_of(a, r);
+  return p.t + 1 < a.L ? a.labels[p.b * a.lb + (p.t + 1) * a.ll] : a.ignore;
+}
 
 template <typename S>
 __device__ __forceinline__ S warp_all_sum(S v) {
@@ -57,14 +72,12 @@ __device__ __forceinline__ S warp_all_sum(S v) {
   return v;
 }
 
-// This CTA's share of the labels that count: those after the first of each sequence that are not ignore_index.
+// This CTA's share of the rows that count.
 __device__ __forceinline__ int64_t count_labels(const LossArgs& a, int64_t cta, int64_t ctas) {
   int64_t n = 0;
-  const int64_t per = a.L - 1, total = a.B * per;
-  for (int64_t e = cta * kThreads + threadIdx.x; e < total; e += ctas * kThreads) {
-    const int64_t b = e / per, t = e - b * per + 1;
-    n += a.labels[b * a.lb + t * a.ll] != a.ignore;
-  }
+  const int64_t rows = a.B * a.L;
+#pragma unroll 4
+  for (int64_t r = cta * blockDim.x + threadIdx.x; r < rows; r += ctas * blockDim.x) n += target_of(a, r) != a.ignore;
   return n;
 }
 
@@ -73,9 +86,15 @@ __device__ __forceinline__ int64_t block_sum_i64(int64_t n, int64_t* ws) {
   if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = n;
   __syncthreads();
   n = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) n += ws[w];
+  for (int w = 0; w < blockDim.x >> 5; ++w) n += ws[w];
   return n;
+}
+
+// All rows that count, the same in every thread.
+__device__ __forceinline__ int64_t total_count(const LossArgs& a, int64_t* ws) {
+  if (!a.counted) return block_sum_i64(count_labels(a, 0, 1), ws);
+  const int lane = threadIdx.x & 31;
+  return warp_all_sum(a.ws->counts[lane] + a.ws->counts[lane + 32]);
 }
 
 __global__ void __launch_bounds__(kThreads) lm_loss_count_kernel(const LossArgs a) {
@@ -84,34 +103,107 @@ __global__ void __launch_bounds__(kThreads) lm_loss_count_kernel(const LossArgs 
   if (threadIdx.x == 0) a.ws->counts[blockIdx.x] = n;
 }
 
-// e^d for d <= 0.
-__device__ __forceinline__ float exp_neg(float d) {
+__device__ __forceinline__ float exp2_fast(float x) {
   float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * kLog2e));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
 
-// (maximum, sum of e^{x - maximum}) of two parts joined; a part without values above -inf is (-inf, 0).
-__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
-  const float top = fmaxf(m, m2);
-  const float f1 = m == top ? 1.f : exp_neg(m - top), f2 = m2 == top ? 1.f : exp_neg(m2 - top);
-  s = s * f1 + s2 * f2;
-  m = top;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
-// 16 bytes of logits as floats.
+// Two 32-bit values an instruction.
+__device__ __forceinline__ uint64_t pair_of(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 split(uint64_t p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^(x log2 e - M) of two values.
+__device__ __forceinline__ uint64_t weight2(uint64_t x, uint64_t neg_m) {
+  const float2 t = split(fma2(x, pair_of(kLog2e, kLog2e), neg_m));
+  return pair_of(exp2_fast(t.x), exp2_fast(t.y));
+}
+
+__device__ __forceinline__ float warp_top(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// A part of a row: M, and the sum of 2^(x log2 e - M) over its values; (-inf, 0) where none is above kLow.
+struct Part {
+  float m, s;
+};
+// The parts of a warp's first kLanes lanes (a power of two) as one, the same in every lane of each kLanes.
+template <int kLanes>
+__device__ __forceinline__ Part join_lanes(Part p) {
+  const float top = warp_top(p.m);
+  p.s *= p.m == top ? 1.f : exp2_fast(p.m - top);  // both may be -inf
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+  p.m = top;
+  return p;
+}
+// The parts of kRow threads as one, the same in each of them; ws is free again after the CTA's next barrier.
+template <int kRow>
+__device__ __forceinline__ Part join_row(Part p, Part* ws) {
+  p = join_lanes<32>(p);
+  if (kRow == 32) return p;
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) ws[threadIdx.x >> 5] = p;
+  __syncthreads();
+  return join_lanes<kRow / 32>(ws[lane % (kRow / 32)]);
+}
+
+// 16 bytes of logits: n values as n / 2 pairs.
 template <typename T>
 struct Piece;
 template <>
 struct Piece<__nv_bfloat16> {
   static constexpr int n = 8;
-  static __device__ __forceinline__ void get(const uint4& r, float* v) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] = __uint_as_float(w[i] << 16);
-      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
+  static __device__ __forceinline__ uint64_t wide(uint32_t w) {
+    return pair_of(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  }
+  static __device__ __forceinline__ void get(const uint4& r, uint64_t* v) {
+    v[0] = wide(r.x);
+    v[1] = wide(r.y);
+    v[2] = wide(r.z);
+    v[3] = wide(r.w);
+  }
+  // A running maximum over pieces, NaN once it has met one.
+  uint32_t w;
+  __device__ __forceinline__ Piece() : w(0xff80ff80u) {}
+  static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+  }
+  __device__ __forceinline__ void meet(const uint4& r) { w = max2(w, max2(max2(r.x, r.y), max2(r.z, r.w))); }
+  __device__ __forceinline__ float top() const {
+    return max_nan(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
   static __device__ __forceinline__ uint4 set(const float* v) {
     uint32_t w[4];
@@ -126,12 +218,17 @@ struct Piece<__nv_bfloat16> {
 template <>
 struct Piece<float> {
   static constexpr int n = 4;
-  static __device__ __forceinline__ void get(const uint4& r, float* v) {
-    v[0] = __uint_as_float(r.x);
-    v[1] = __uint_as_float(r.y);
-    v[2] = __uint_as_float(r.z);
-    v[3] = __uint_as_float(r.w);
+  static __device__ __forceinline__ void get(const uint4& r, uint64_t* v) {
+    v[0] = pair_of(__uint_as_float(r.x), __uint_as_float(r.y));
+    v[1] = pair_of(__uint_as_float(r.z), __uint_as_float(r.w));
   }
+  float m;
+  __device__ __forceinline__ Piece() : m(-INFINITY) {}
+  __device__ __forceinline__ void meet(const uint4& r) {
+    m = max_nan(m, max_nan(max_nan(__uint_as_float(r.x), __uint_as_float(r.y)),
+                           max_nan(__uint_as_float(r.z), __uint_as_float(r.w))));
+  }
+  __device__ __forceinline__ float top() const { return m; }
   static __device__ __forceinline__ uint4 set(const float* v) {
     return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
   }
@@ -153,27 +250,52 @@ struct Walk {
   __device__ __forceinline__ int edge(int e) const { return e < first ? e : V - edges + e; }  // e < edges
 };
 
-// Adds a value to the thread's running (m, s).
-__device__ __forceinline__ void add_value(float& m, float& s, float v) {
-  if (v > m) {
-    s *= exp_neg(m - v);
-    m = v;
+// Sum or maximum over the threads of a row, the same value in each of them; ws is free on entry and on return.
+template <int kRow, bool kMax>
+__device__ __forceinline__ float row_reduce(float v, float* ws) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(0xffffffffu, v, o);
+    v = kMax ? fmaxf(v, w) : v + w;
   }
-  if (v != -INFINITY) s += exp_neg(v - m);
+  if (kRow == 32) return v;
+  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = ws[0];
+#pragma unroll
+  for (int w = 1; w < kRow / 32; ++w) v = kMax ? fmaxf(v, ws[w]) : v + ws[w];
+  __syncthreads();
+  return v;
+}
+
+// A row with no value above kLow, by differences first, a value at a time; the gradient of its values i0 .. i1 - 1.  Rows
+// of -inf alone come out NaN.
+template <typename T, int kRow>
+__device__ __noinline__ float low_row(const T* x, T* g, int V, int i0, int i1, int target, int lane, float inv_count,
+                                      float* ws) {
+  if (kRow > 32) __syncthreads();  // ws has been read
+  float m = -INFINITY, s = 0.f;
+  for (int i = lane; i < V; i += kRow) m = fmaxf(m, to_float(x[i]));
+  m = row_reduce<kRow, true>(m, ws);
+  for (int i = lane; i < V; i += kRow) s += expf(to_float(x[i]) - m);
+  s = row_reduce<kRow, false>(s, ws);
+  if (g)
+    for (int i = i0 + lane; i < i1; i += kRow)
+      g[i] = from_float<T>(expf(to_float(x[i]) - m) * (inv_count / s) - (i == target ? inv_count : 0.f));
+  return logf(s) - (to_float(x[target]) - m);
 }
 
 // A row by kRow threads (a warp, or the CTA); lane: the thread's number among them.  Returns the row's loss.
-template <typename T, int kRow>
-__device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int lane, float inv_count, float* m_ws,
-                                          float* s_ws) {
-  constexpr int n = Piece<T>::n, kAhead = 4;
-  const int64_t b = r / a.L, t = r - b * a.L;
-  const T* x = static_cast<const T*>(a.logits) + b * a.xb + t * a.xl;
-  T* g = a.grad ? static_cast<T*>(a.grad) + b * a.gb + t * a.gl : nullptr;
+template <typename T, int kRow, int kAhead>
+__device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
+                                          Part* ws) {
+  constexpr int n = Piece<T>::n;
+  const Position pos = position_of(a, r);
+  const T* x = static_cast<const T*>(a.logits) + pos.b * a.xb + pos.t * a.xl;
+  T* g = a.grad ? static_cast<T*>(a.grad) + pos.b * a.gb + pos.t * a.gl : nullptr;
   const Walk walk(x, g, (int)a.V);
   const uint4* xp = reinterpret_cast<const uint4*>(x + walk.first);
   uint4* gp = reinterpret_cast<uint4*>(g + walk.first);
-  const int64_t target = t + 1 < a.L ? a.labels[b * a.lb + (t + 1) * a.ll] : a.ignore;
   if (target == a.ignore) {
     if (g) {
       for (int i = lane; i < walk.pieces; i += kRow) __stcs(gp + i, make_uint4(0, 0, 0, 0));
@@ -181,118 +303,142 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int lane
     }
     return 0.f;
   }
+  const float nan = __int_as_float(0x7fc00000);
   const bool bad = target < 0 || target >= a.V;
   if (bad && lane == 0) set_error(a.err, GSA_ERR_INDEX);
-  float m = -INFINITY, s = 0.f;
+  const float x_target = bad ? nan : to_float(x[target]);
+  const bool once = walk.pieces <= kAhead * kRow;  // the pieces stay in registers between the passes
+  float top = -INFINITY;  // the thread's largest value
+  Part p{-INFINITY, 0.f};
+  uint4 raw[kAhead];
   for (int i0 = lane; i0 < walk.pieces; i0 += kAhead * kRow) {
-    uint4 raw[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (i0 + j * kRow < walk.pieces) raw[j] = xp[i0 + j * kRow];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j * kRow >= walk.pieces) break;
-      float v[n];
-      Piece<T>::get(raw[j], v);
-      float top = v[0];
-#pragma unroll
-      for (int k = 1; k < n; ++k) top = fmaxf(top, v[k]);
-      if (top > m) {
-        s *= exp_neg(m - top);
-        m = top;
+      Piece<T> most;
+      most.meet(raw[j]);
+      const float here = most.top();
+      if (here <= kLow) continue;
+      if (here > top) {
+        top = here;
+        const float up = here * kLog2e;
+        p.s *= exp2_fast(p.m - up);
+        p.m = up;
       }
-      if (top == -INFINITY) continue;  // all of them masked: their weight is 0, and m may be -inf still
+      uint64_t v[n / 2];
+      Piece<T>::get(raw[j], v);
+      const uint64_t neg_m = pair_of(-p.m, -p.m);
+      uint64_t sum = weight2(v[0], neg_m);
 #pragma unroll
-      for (int k = 0; k < n; ++k) s += exp_neg(v[k] - m);
+      for (int k = 1; k < n / 2; ++k) sum = add2(sum, weight2(v[k], neg_m));
+      const float2 both = split(sum);
+      p.s += both.x + both.y;
     }
   }
-  for (int e = lane; e < walk.edges; e += kRow) add_value(m, s, to_float(x[walk.edge(e)]));
-  for (int o = 16; o > 0; o >>= 1)
-    join(m, s, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o));
-  if (kRow > 32) {
-    __syncthreads();  // the last row's parts have been read
-    if ((threadIdx.x & 31) == 0) {
-      m_ws[threadIdx.x >> 5] = m;
-      s_ws[threadIdx.x >> 5] = s;
+  for (int e = lane; e < walk.edges; e += kRow) {
+    const float v = to_float(x[walk.edge(e)]);
+    if (v <= kLow) continue;
+    if (v > top) {
+      top = v;
+      p.s *= exp2_fast(p.m - v * kLog2e);
+      p.m = v * kLog2e;
     }
-    __syncthreads();
-    m = m_ws[0];
-    s = s_ws[0];
-#pragma unroll
-    for (int w = 1; w < kRow / 32; ++w) join(m, s, m_ws[w], s_ws[w]);
+    p.s += exp2_fast(fmaf(v, kLog2e, -p.m));
   }
+  p = join_row<kRow>(p, ws);
+  const float m = p.m, s = p.s;
+  if (m == -INFINITY && s == 0.f && !bad)
+    return low_row<T, kRow>(x, g, walk.V, 0, walk.V, (int)target, lane, inv_count, &ws[0].m);
   // a label out of range, a NaN or a logit of +inf: the row's loss and gradient are NaN
-  const float d = bad || m == INFINITY ? __int_as_float(0x7fc00000) : m - to_float(x[target]);
-  const float loss = d + logf(s);
+  const float loss = bad || m == INFINITY ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
   if (!g) return loss;
   const float inv = isnan(loss) ? loss : inv_count / s;
-  const int at = (int)target - walk.first;  // in 16-byte pieces' values
+  const int at = bad ? -1 : (int)target - walk.first;  // in 16-byte pieces' values
+  const uint64_t neg_m = pair_of(-m, -m), inv2 = pair_of(inv, inv);
   for (int i0 = lane; i0 < walk.pieces; i0 += kAhead * kRow) {
-    uint4 raw[kAhead];
+    if (!once) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (i0 + j * kRow < walk.pieces) raw[j] = __ldcs(xp + i0 + j * kRow);
+      for (int j = 0; j < kAhead; ++j)
+        if (i0 + j * kRow < walk.pieces) raw[j] = __ldcs(xp + i0 + j * kRow);
+    }
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       const int i = i0 + j * kRow;
       if (i >= walk.pieces) break;
-      float v[n];
+      uint64_t v[n / 2];
       Piece<T>::get(raw[j], v);
+      float q[n];
 #pragma unroll
-      for (int k = 0; k < n; ++k) v[k] = exp_neg(v[k] - m) * inv;
+      for (int k = 0; k < n / 2; ++k) {
+        const float2 both = split(mul2(weight2(v[k], neg_m), inv2));
+        q[2 * k] = both.x;
+        q[2 * k + 1] = both.y;
+      }
       const int k0 = at - i * n;
       if (k0 >= 0 && k0 < n) {
 #pragma unroll
         for (int k = 0; k < n; ++k)
-          if (k == k0) v[k] -= inv_count;
+          if (k == k0) q[k] -= inv_count;
       }
-      __stcs(gp + i, Piece<T>::set(v));
+      __stcs(gp + i, Piece<T>::set(q));
     }
   }
   for (int e = lane; e < walk.edges; e += kRow) {
     const int i = walk.edge(e);
-    float p = exp_neg(to_float(x[i]) - m) * inv;
-    if (i == (int)target) p -= inv_count;
-    g[i] = from_float<T>(p);
+    float q = exp2_fast(fmaf(to_float(x[i]), kLog2e, -m)) * inv;
+    if (i == (int)target) q -= inv_count;
+    g[i] = from_float<T>(q);
   }
   return loss;
 }
 
-template <typename T, int kRow>
-__global__ void __launch_bounds__(kThreads, kPerSm) lm_loss_kernel(const LossArgs a) {
-  __shared__ int64_t cnt_ws[kWarps];
-  __shared__ float m_ws[kWarps], s_ws[kWarps];
-  __shared__ double sum_ws[kWarps];
+// kThreads threads, kRow a row; a row's label is loaded while the one before it is worked on.
+template <typename T, int kRow, int kCta, int kCtas, int kAhead>
+__global__ void __launch_bounds__(kCta, kCtas) lm_loss_kernel(const LossArgs a) {
+  constexpr int kRows = kCta / kRow, kW = kCta / 32;
+  __shared__ int64_t cnt_ws[kW];
+  __shared__ Part row_ws[2][kW];
+  __shared__ double sum_ws[kW];
   chain_wait();
-  int64_t count = 0;
-  if (a.counted) {
-    for (int i = 0; i < kCounters; ++i) count += a.ws->counts[i];
-  } else {
-    count = block_sum_i64(count_labels(a, 0, 1), cnt_ws);
-  }
+  int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kRow;
+  const int64_t step = (int64_t)gridDim.x * kRows, rows = a.B * a.L;
+  int64_t target = target_of(a, r);
+  const int64_t count = total_count(a, cnt_ws);
   if (blockIdx.x == 0 && threadIdx.x == 0) a.ws->count = count;
   const float inv_count = count ? 1.0f / (float)count : 0.f;
-  constexpr int kRows = kThreads / kRow;
-  const int64_t rows = a.B * a.L;
   double sum = 0;
-  for (int64_t r = (int64_t)blockIdx.x * kRows + threadIdx.x / kRow; r < rows; r += (int64_t)gridDim.x * kRows)
-    sum += row_loss<T, kRow>(a, r, threadIdx.x % kRow, inv_count, m_ws, s_ws);
+  // two of row_ws in turn: a row's barrier is what frees the one before it
+  for (int turn = 0; r < rows; r += step) {
+    const int64_t next = target_of(a, r + step);
+    sum += row_loss<T, kRow, kAhead>(a, r, target, threadIdx.x % kRow, inv_count, row_ws[turn]);
+    if (target != a.ignore) turn ^= 1;
+    target = next;
+  }
   if (kRow == 32) {
     if ((threadIdx.x & 31) == 0) sum_ws[threadIdx.x >> 5] = sum;
     __syncthreads();
     sum = 0;
-    for (int w = 0; w < kWarps; ++w) sum += sum_ws[w];
+    for (int w = 0; w < kW; ++w) sum += sum_ws[w];
   }
   if (threadIdx.x == 0) a.ws->sums[blockIdx.x] = sum;
 }
 
 // The mean of the rows' losses: NaN where no label counts (0 / 0).
-__global__ void __launch_bounds__(32) lm_loss_mean_kernel(const LossArgs a, int parts) {
+__global__ void __launch_bounds__(256) lm_loss_mean_kernel(const LossArgs a, int parts) {
+  __shared__ double ws[8];
   chain_wait();
   double sum = 0;
-  for (int i = threadIdx.x; i < parts; i += 32) sum += a.ws->sums[i];
+  for (int i = threadIdx.x; i < parts; i += 256) sum += a.ws->sums[i];
   sum = warp_all_sum(sum);
-  if (threadIdx.x == 0) *a.loss = (float)(sum / (double)(parts ? a.ws->count : 0));
+  if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = sum;
+  __syncthreads();
+  if (threadIdx.x) return;
+  sum = 0;
+  for (int w = 0; w < 8; ++w) sum += ws[w];
+  *a.loss = (float)(sum / (double)(parts ? a.ws->count : 0));
 }
 
 template <typename T>
@@ -303,15 +449,27 @@ __global__ void __launch_bounds__(256) scale_kernel(int64_t n, T* x, const float
     x[i] = from_float<T>(to_float(x[i]) * f);
 }
 
-template <typename T>
+template <typename T, int kRow, int kCta, int kCtas, int kAhead>
 cudaError_t launch_rows(const LossArgs& a, int* grid, cudaStream_t s) {
-  const int64_t rows = a.B * a.L;
-  if (a.V <= kWarpRow) {
-    *grid = (int)std::min<int64_t>((rows + kWarps - 1) / kWarps, 148 * kPerSm);
-    return launch_chained(lm_loss_kernel<T, 32>, *grid, kThreads, 0, s, a);
-  }
-  *grid = (int)std::min<int64_t>(rows, 148 * kPerSm);
-  return launch_chained(lm_loss_kernel<T, kThreads>, *grid, kThreads, 0, s, a);
+  constexpr int kRows = kCta / kRow;
+  *grid = (int)std::min<int64_t>((a.B * a.L + kRows - 1) / kRows, 148 * kCtas);
+  return launch_chained(lm_loss_kernel<T, kRow, kCta, kCtas, kAhead>, *grid, kCta, 0, s, a);
+}
+
+// Threads a row: 1024 threads an SM in any case, on as many rows as their second reading finds in L2 -- 16 rows an SM of
+// up to 20 KB (48 MB in flight), 8 of up to 48 KB, 4 of up to 112 KB, 2 of up to 320 KB, then 1.  Measured in TB/s with
+// twice the threads a row | as here | with half: 8 KB rows 4.1 | 4.6 | -, 40 KB 4.8 | 5.1 | 4.6, 98 KB 4.6 | 4.8 | 4.4,
+// 250 KB 4.9 | 5.0 | 4.4, 501 KB (fp32) - | 5.1 | 4.5.
+template <typename T>
+cudaError_t launch_loss(const LossArgs& a, int* grid, cudaStream_t s) {
+  const int64_t bytes = a.V * (int64_t)sizeof(T);
+  if (bytes <= 1024) return launch_rows<T, 32, 256, 6, 2>(a, grid, s);
+  if (bytes <= 4096) return launch_rows<T, 32, 256, 4, 8>(a, grid, s);
+  if (bytes <= 20 << 10) return launch_rows<T, 64, 64, 16, 6>(a, grid, s);
+  if (bytes <= 48 << 10) return launch_rows<T, 128, 128, 8, 6>(a, grid, s);
+  if (bytes <= 112 << 10) return launch_rows<T, 256, 256, 4, 6>(a, grid, s);
+  if (bytes <= 320 << 10) return launch_rows<T, 512, 512, 2, 6>(a, grid, s);
+  return launch_rows<T, 1024, 1024, 1, 6>(a, grid, s);
 }
 
 }  // namespace
@@ -336,7 +494,8 @@ int gsa_next_token_loss(int dtype, int64_t B, int64_t L, int64_t V, const void* 
   if (!workspace || workspace_bytes < (int64_t)sizeof(Workspace) || reinterpret_cast<uintptr_t>(workspace) % 16)
     return GSA_ERR_WORKSPACE;
   LossArgs a{B, L, V, logits, x_bstride, x_lstride, labels, lab_bstride, lab_lstride, ignore_index,
-             static_cast<Workspace*>(workspace), grad, g_bstride, g_lstride, loss, nullptr, rows > kSelfCount};
+             static_cast<Workspace*>(workspace), grad, g_bstride, g_lstride, loss, nullptr, rows > kSelfCount,
+             L > 1 ? ~0ull / (uint64_t)L + 1 : 0};
   int st = device_error_word(&a.err);
   if (st) return st;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
@@ -346,11 +505,11 @@ int gsa_next_token_loss(int dtype, int64_t B, int64_t L, int64_t V, const void* 
       lm_loss_count_kernel<<<kCounters, kThreads, 0, s>>>(a);
       if (cudaGetLastError() != cudaSuccess) return GSA_ERR_LAUNCH;
     }
-    const cudaError_t e = dtype == GSA_DTYPE_BF16 ? launch_rows<__nv_bfloat16>(a, &grid, s)
-                                                  : launch_rows<float>(a, &grid, s);
+    const cudaError_t e = dtype == GSA_DTYPE_BF16 ? launch_loss<__nv_bfloat16>(a, &grid, s)
+                                                  : launch_loss<float>(a, &grid, s);
     if (e != cudaSuccess) return GSA_ERR_LAUNCH;
   }
-  return launch_chained(lm_loss_mean_kernel, 1, 32, 0, s, a, grid) == cudaSuccess ? GSA_OK : GSA_ERR_LAUNCH;
+  return launch_chained(lm_loss_mean_kernel, 1, 256, 0, s, a, grid) == cudaSuccess ? GSA_OK : GSA_ERR_LAUNCH;
 }
 
 int gsa_scale(int dtype, int64_t n, void* x, const float* factor, gsa_stream_t stream) {

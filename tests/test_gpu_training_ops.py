@@ -467,7 +467,8 @@ def _loss_oracle(logits, labels, ignore=-100):
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("B,L,V", [(1, 2, 1), (1, 2, 2), (2, 96, 384), (3, 17, 1000), (1, 33, 4097), (2, 5, 128256), (1, 600, 31),
-                                   (1, 3, 32768), (700, 2, 8), (1, 9, 50257)])
+                                   (1, 3, 32768), (700, 2, 8), (1, 9, 50257), (2, 200, 32768), (1, 3, 20000),
+                                   (1, 150, 65544), (1, 3, 131072), (1, 2, 262152)])
 def test_loss_and_gradient(cuda_ok, dtype, B, L, V):
     import gsa_b200 as gsa
 
@@ -503,13 +504,13 @@ def test_loss_gradient_is_that_of_differences(cuda_ok):
     assert abs(float((grad.double() * v).sum() - (up - down) / (2 * e))) < 400 * 16 * U
 
 
-def test_loss_special_rows(cuda_ok):
+@pytest.mark.parametrize("V", [70, 3000, 4099, 32768, 65536, 128256])
+def test_loss_special_rows(cuda_ok, V):
     """Masked (-inf) logits, a target among them, large and equal logits, rows that do not count, no row that counts, another
     ignore_index, a label out of range, NaN."""
     import gsa_b200 as gsa
     from gsa_b200 import _lib, ops
 
-    V = 70
     x = _randn(1, 1, 6, V)
     x[0, 0, 5:60] = -math.inf
     x[0, 1] = 1000.0
@@ -518,8 +519,9 @@ def test_loss_special_rows(cuda_ok):
     labels = torch.tensor([[9, 2, 3, 4, 0, 64]], device=DEV)
     want, g, size, far, loss_size = _loss_oracle(x, labels)
     loss, grad = ops.next_token_loss(x, labels)
-    _near(loss, want, 64 * U * (1 + loss_size))
-    _near(grad, g, size * 256 * U)
+    # a sum of V terms (V / 32 additions after one another at most), and 2^(x log2 e - M) at |x| of 1000: 256 U
+    _near(loss, want, (V / 32 + 64) * U * (1 + loss_size))
+    _near(grad, g, size * (V / 32 + 256) * U)
     assert bool((grad[0, 0, 5:60] == 0).all()) and bool((grad[0, 5] == 0).all())
     # the target itself masked: an infinite loss, a finite gradient
     hit = labels.clone()
@@ -532,13 +534,30 @@ def test_loss_special_rows(cuda_ok):
         assert bool(torch.isnan(loss)) and bool((grad == 0).all())
     loss, grad = ops.next_token_loss(x[:, :1], labels[:, :1])
     assert bool(torch.isnan(loss)) and bool((grad == 0).all())
-    # NaN and +inf stay in their rows
+    # NaN and +inf take their row, a NaN among masked values too, and no other
     for bad in (math.nan, math.inf):
-        y = x.clone()
-        y[0, 1, 3] = bad
+        for row, at in ((1, 3), (0, 30), (0, V - 1)):
+            y = x.clone()
+            y[0, row, at] = bad
+            loss, grad = ops.next_token_loss(y, labels)
+            assert bool(torch.isnan(loss)) and bool(torch.isnan(grad[0, row]).all()), (bad, row, at)
+            assert bool(torch.isfinite(grad[0, [r for r in range(6) if r != row]]).all())
+    # rows masked throughout: the type's lowest value is as good as any other, -inf is not
+    for dtype in (torch.float32, torch.bfloat16):
+        y = x.to(dtype, copy=True)
+        y[0, 2] = torch.finfo(dtype).min
+        y[0, 4, ::2] = torch.finfo(dtype).min
+        y[0, 4, 1::2] = -math.inf
         loss, grad = ops.next_token_loss(y, labels)
-        assert bool(torch.isnan(loss)) and bool(torch.isnan(grad[0, 1]).all())
-        assert bool(torch.isfinite(grad[0, [0, 2, 3, 4, 5]]).all())
+        assert bool(torch.isfinite(loss)) and bool(torch.isfinite(grad[0, [0, 1, 2, 3]]).all())
+        even = torch.arange(V, device=DEV) % 2 == 0
+        for row, p, on in ((2, 1 / V, torch.ones_like(even)), (4, 1 / ((V + 1) // 2), even)):
+            want = torch.where(on, p, 0.0).double()
+            want[labels[0, row + 1]] -= 1
+            _near(grad[0, row], want / 5, 16 * U * (want.abs() + p) / 5)
+        y[0, 3] = -math.inf
+        loss, grad = ops.next_token_loss(y, labels)
+        assert bool(torch.isnan(loss)) and bool(torch.isnan(grad[0, 3]).all()) and bool(torch.isfinite(grad[0, 4]).all())
     ops.check_device_error()
     wrong = labels.clone()
     wrong[0, 2] = V
