@@ -4,7 +4,7 @@
 //   loss = mean over the counted positions of (log sum_v e^{x_v} - x_target)
 //   grad = (softmax(x) - onehot(target)) / count, zero in the rows that do not count
 //
-// A CTA takes a row (a warp takes one of up to 4 KB): its maximum and sum in one pass (online), then the gradient
+// A CTA takes a row (a warp one of up to 4 KB, eight lanes one of up to 1 KB): its maximum and sum in one pass (online), then the gradient
 // from a second reading, which registers serve for short rows and the L2 for long ones: the rows in flight are up to
 // 76 MB.  So HBM sees each logit about once (1.1 times for rows of 250 KB) and each gradient value once.
 // Exponentials are 2^(x log2 e - M) by one multiply-add (two values an instruction) and one ex2, M the rounded m log2 e:
@@ -157,25 +157,37 @@ __device__ __forceinline__ float warp_top(float v) {
 struct Part {
   float m, s;
 };
-// The parts of a warp's first kLanes lanes (a power of two) as one, the same in every lane of each kLanes.
+// The lanes of this thread's row, where a warp holds rows of kRow lanes.
+template <int kRow>
+__device__ __forceinline__ uint32_t row_mask() {
+  return kRow >= 32 ? 0xffffffffu : ((1u << (kRow & 31)) - 1u) << ((threadIdx.x & 31) / kRow * kRow);
+}
+// The parts of kLanes neighbouring lanes (a power of two) as one, the same in each of them.
 template <int kLanes>
 __device__ __forceinline__ Part join_lanes(Part p) {
-  const float top = warp_top(p.m);
+  float top = p.m;
+  if (kLanes >= 16) {  // of all the warp: the lanes beside hold the same parts
+    top = warp_top(top);
+  } else {
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(row_mask<kLanes>(), top, o));
+  }
   p.s *= p.m == top ? 1.f : exp2_fast(p.m - top);  // both may be -inf
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) p.s += __shfl_xor_sync(0xffffffffu, p.s, o);
+  for (int o = kLanes / 2; o > 0; o >>= 1) p.s += __shfl_xor_sync(row_mask<kLanes>(), p.s, o);
   p.m = top;
   return p;
 }
 // The parts of kRow threads as one, the same in each of them; ws is free again after the CTA's next barrier.
 template <int kRow>
 __device__ __forceinline__ Part join_row(Part p, Part* ws) {
+  if (kRow <= 32) return join_lanes<(kRow < 32 ? kRow : 32)>(p);
   p = join_lanes<32>(p);
-  if (kRow == 32) return p;
+  constexpr int kParts = kRow < 64 ? 1 : kRow / 32;
   const int lane = threadIdx.x & 31;
   if (lane == 0) ws[threadIdx.x >> 5] = p;
   __syncthreads();
-  return join_lanes<kRow / 32>(ws[lane % (kRow / 32)]);
+  return join_lanes<kParts>(ws[lane % kParts]);
 }
 
 // 16 bytes of logits: n values as n / 2 pairs.
@@ -254,11 +266,11 @@ struct Walk {
 template <int kRow, bool kMax>
 __device__ __forceinline__ float row_reduce(float v, float* ws) {
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float w = __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = (kRow < 32 ? kRow : 32) / 2; o > 0; o >>= 1) {
+    const float w = __shfl_xor_sync(row_mask<kRow>(), v, o);
     v = kMax ? fmaxf(v, w) : v + w;
   }
-  if (kRow == 32) return v;
+  if (kRow <= 32) return v;
   if ((threadIdx.x & 31) == 0) ws[threadIdx.x >> 5] = v;
   __syncthreads();
   v = ws[0];
@@ -285,7 +297,7 @@ __device__ __noinline__ float low_row(const T* x, T* g, int V, int i0, int i1, i
   return logf(s) - (to_float(x[target]) - m);
 }
 
-// A row by kRow threads (a warp, or the CTA); lane: the thread's number among them.  Returns the row's loss.
+// A row by kRow threads (neighbouring lanes, or the CTA); lane: the thread's number among them.  Returns the row's loss.
 template <typename T, int kRow, int kAhead>
 __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
                                           Part* ws) {
@@ -417,7 +429,9 @@ __global__ void __launch_bounds__(kCta, kCtas) lm_loss_kernel(const LossArgs a) 
     if (target != a.ignore) turn ^= 1;
     target = next;
   }
-  if (kRow == 32) {
+  if (kRow <= 32) {
+#pragma unroll
+    for (int o = kRow; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if ((threadIdx.x & 31) == 0) sum_ws[threadIdx.x >> 5] = sum;
     __syncthreads();
     sum = 0;
@@ -463,7 +477,7 @@ cudaError_t launch_rows(const LossArgs& a, int* grid, cudaStream_t s) {
 template <typename T>
 cudaError_t launch_loss(const LossArgs& a, int* grid, cudaStream_t s) {
   const int64_t bytes = a.V * (int64_t)sizeof(T);
-  if (bytes <= 1024) return launch_rows<T, 32, 256, 6, 2>(a, grid, s);
+  if (bytes <= 1024) return launch_rows<T, 8, 256, 4, 8>(a, grid, s);
   if (bytes <= 4096) return launch_rows<T, 32, 256, 4, 8>(a, grid, s);
   if (bytes <= 20 << 10) return launch_rows<T, 64, 64, 16, 6>(a, grid, s);
   if (bytes <= 48 << 10) return launch_rows<T, 128, 128, 8, 6>(a, grid, s);

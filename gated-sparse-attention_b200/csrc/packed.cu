@@ -8,7 +8,7 @@
 //
 // Products are in 32 bits; an output is rounded once, to its type.  All are bound by the bytes that they move, so
 // a thread holds 16 neighbouring values (half a group, 32-byte loads and stores, one shuffle for the scale) wherever
-// the rows are whole multiples of that and aligned; rows that are not take a value a lane (a group a warp).
+// the rows are whole multiples of that and aligned; rows that are not take a value a lane, four groups a warp.
 #include <algorithm>
 
 #include "packed.cuh"
@@ -40,7 +40,7 @@ __device__ __forceinline__ SwigluGrad swiglu_grad(float dz, float g, float u) {
 // neighbouring lanes; the last may be empty.
 // ---------------------------------------------------------------------------------------------
 struct Cut {
-  int64_t rows, halves, per_row;  // halves: rows * per_row
+  int64_t rows, halves, per_row;  // halves (or spans): rows * per_row
   uint64_t magic;
   int64_t n;
 };
@@ -137,91 +137,120 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // ---------------------------------------------------------------------------------------------
-// A value a lane.
+// A value a lane, kLaneGroups groups of a row a warp.
 // ---------------------------------------------------------------------------------------------
+constexpr int kLaneGroups = 4;
+constexpr int kSpan = kLaneGroups * kGroup;
+
+// The warp's row and the lane's first value in it; false past the last.
+__device__ __forceinline__ bool span_of(const Cut& c, int64_t* r, int64_t* i) {
+  const int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (w >= c.halves) return false;
+  *r = c.per_row == 1 ? w : row_of(w, c.magic);
+  *i = (w - *r * c.per_row) * kSpan + (threadIdx.x & 31);
+  return true;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) pack_kernel(int64_t rows, int64_t n, const T* x, int64_t x_ld,
-                                                        uint8_t* codes, int64_t c_ld, uint8_t* scales, int64_t s_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t g = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); g < total; g += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = g / groups, i = (g - r * groups) * kGroup + lane;
+__global__ void __launch_bounds__(kThreads) pack_kernel(const Cut c, const T* x, int64_t x_ld, uint8_t* codes,
+                                                        int64_t c_ld, uint8_t* scales, int64_t s_ld) {
+  int64_t r, i;
+  if (!span_of(c, &r, &i)) return;
+  float v[kLaneGroups];
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) v[k] = i + k * kGroup < c.n ? to_float(x[r * x_ld + i + k * kGroup]) : 0.f;
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) {
     int s;
-    const uint32_t c = pack_lane(i < n ? to_float(x[r * x_ld + i]) : 0.f, &s);
-    if (i < n) codes[r * c_ld + i] = (uint8_t)c;
-    if (lane == 0) scales[r * s_ld + i / kGroup] = (uint8_t)s;
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) unpack_kernel(int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld,
-                                                          const uint8_t* scales, int64_t s_ld, T* x, int64_t x_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t g = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); g < total; g += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = g / groups, i = (g - r * groups) * kGroup + lane;
-    if (i < n) x[r * x_ld + i] = from_float<T>(unpack_one(codes[r * c_ld + i], scales[r * s_ld + i / kGroup]));
-  }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(int64_t rows, int64_t n, const T* gu, int64_t gu_ld,
-                                                                 T* z, int64_t z_ld, uint8_t* codes, int64_t c_ld,
-                                                                 uint8_t* scales, int64_t s_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); w < total; w += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = w / groups, i = (w - r * groups) * kGroup + lane;
-    const float g = i < n ? to_float(gu[r * gu_ld + i]) : 0.f;
-    const float u = i < n ? to_float(gu[r * gu_ld + n + i]) : 0.f;
-    int sg, su;
-    const uint32_t cg = pack_lane(g, &sg), cu = pack_lane(u, &su);
-    if (i < n) {
-      z[r * z_ld + i] = from_float<T>(g * sigmoid32(g) * u);
-      codes[2 * r * c_ld + i] = (uint8_t)cg;
-      codes[(2 * r + 1) * c_ld + i] = (uint8_t)cu;
+    const uint32_t q = pack_lane(v[k], &s);  // by all lanes, in a group beyond the row too
+    if (i + k * kGroup < c.n) {
+      codes[r * c_ld + i + k * kGroup] = (uint8_t)q;
+      if ((threadIdx.x & 31) == 0) scales[r * s_ld + i / kGroup + k] = (uint8_t)s;
     }
-    if (lane == 0) {
-      scales[2 * r * s_ld + i / kGroup] = (uint8_t)sg;
-      scales[(2 * r + 1) * s_ld + i / kGroup] = (uint8_t)su;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) unpack_kernel(const Cut c, const uint8_t* codes, int64_t c_ld,
+                                                          const uint8_t* scales, int64_t s_ld, T* x, int64_t x_ld) {
+  int64_t r, i;
+  if (!span_of(c, &r, &i)) return;
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k)
+    if (i + k * kGroup < c.n)
+      x[r * x_ld + i + k * kGroup] =
+          from_float<T>(unpack_one(codes[r * c_ld + i + k * kGroup], scales[r * s_ld + i / kGroup + k]));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(const Cut c, const T* gu, int64_t gu_ld, T* z,
+                                                                 int64_t z_ld, uint8_t* codes, int64_t c_ld,
+                                                                 uint8_t* scales, int64_t s_ld) {
+  int64_t r, i;
+  if (!span_of(c, &r, &i)) return;
+  float g[kLaneGroups], u[kLaneGroups];
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) {
+    const bool live = i + k * kGroup < c.n;
+    g[k] = live ? to_float(gu[r * gu_ld + i + k * kGroup]) : 0.f;
+    u[k] = live ? to_float(gu[r * gu_ld + c.n + i + k * kGroup]) : 0.f;
+  }
+  auto* cp = codes + 2 * r * c_ld + i;
+  auto* sp = scales + 2 * r * s_ld + i / kGroup;
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) {
+    int sg, su;
+    const uint32_t cg = pack_lane(g[k], &sg), cu = pack_lane(u[k], &su);  // by all lanes
+    if (i + k * kGroup < c.n) {
+      z[r * z_ld + i + k * kGroup] = from_float<T>(g[k] * sigmoid32(g[k]) * u[k]);
+      cp[k * kGroup] = (uint8_t)cg;
+      cp[c_ld + k * kGroup] = (uint8_t)cu;
+      if ((threadIdx.x & 31) == 0) {
+        sp[k] = (uint8_t)sg;
+        sp[s_ld + k] = (uint8_t)su;
+      }
     }
   }
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
-    silu_mul_bwd_kernel(int64_t rows, int64_t n, const T* dz, int64_t dz_ld, const uint8_t* codes, int64_t c_ld,
+    silu_mul_bwd_kernel(const Cut c, const T* dz, int64_t dz_ld, const uint8_t* codes, int64_t c_ld,
                         const uint8_t* scales, int64_t s_ld, T* dgu, int64_t dgu_ld, T* z, int64_t z_ld) {
-  const int64_t groups = (n + kGroup - 1) / kGroup, total = rows * groups;
-  const int lane = threadIdx.x & 31;
-  for (int64_t w = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5); w < total; w += (int64_t)gridDim.x * kWarps) {
-    const int64_t r = w / groups, i = (w - r * groups) * kGroup + lane, r2 = 2 * r;
-    if (i >= n) continue;
-    const float g = unpack_one(codes[r2 * c_ld + i], scales[r2 * s_ld + i / kGroup]);
-    const float u = unpack_one(codes[(r2 + 1) * c_ld + i], scales[(r2 + 1) * s_ld + i / kGroup]);
-    const SwigluGrad d = swiglu_grad(to_float(dz[r * dz_ld + i]), g, u);
-    dgu[r * dgu_ld + i] = from_float<T>(d.dg);
-    dgu[r * dgu_ld + n + i] = from_float<T>(d.du);
-    if (z) z[r * z_ld + i] = from_float<T>(d.z);
+  int64_t r, i;
+  if (!span_of(c, &r, &i)) return;
+  auto* cp = codes + 2 * r * c_ld + i;
+  auto* sp = scales + 2 * r * s_ld + i / kGroup;
+  float d[kLaneGroups], g[kLaneGroups], u[kLaneGroups];
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) {
+    if (i + k * kGroup >= c.n) break;
+    d[k] = to_float(dz[r * dz_ld + i + k * kGroup]);
+    g[k] = unpack_one(cp[k * kGroup], sp[k]);
+    u[k] = unpack_one(cp[c_ld + k * kGroup], sp[s_ld + k]);
+  }
+#pragma unroll
+  for (int k = 0; k < kLaneGroups; ++k) {
+    const int64_t at = i + k * kGroup;
+    if (at >= c.n) break;
+    const SwigluGrad q = swiglu_grad(d[k], g[k], u[k]);
+    dgu[r * dgu_ld + at] = from_float<T>(q.dg);
+    dgu[r * dgu_ld + c.n + at] = from_float<T>(q.du);
+    if (z) z[r * z_ld + at] = from_float<T>(q.z);
   }
 }
 
-// One CTA per 256 halves; the sizes that a grid cannot hold (beyond 2^31 CTAs: 2^43 values) are refused.
-bool cut(int64_t rows, int64_t n, Cut* c, unsigned* grid) {
+// Rows cut into halves of groups, one a thread, or into spans of kLaneGroups groups, one a warp.  False where a
+// grid cannot hold them (beyond 2^31 CTAs: 2^41 values).
+bool cut(int64_t rows, int64_t n, bool halves, Cut* c, unsigned* grid) {
   c->rows = rows;
   c->n = n;
-  c->per_row = (n + kGroup - 1) / kGroup * 2;
+  c->per_row = halves ? (n + kGroup - 1) / kGroup * 2 : (n + kSpan - 1) / kSpan;
   c->halves = rows * c->per_row;
-  c->magic = row_magic(rows, c->per_row);
-  const int64_t blocks = (c->halves + kThreads - 1) / kThreads;
+  c->magic = c->per_row == 1 ? 0 : row_magic(rows, c->per_row);
+  const int64_t each = halves ? kThreads : kWarps, blocks = (c->halves + each - 1) / each;
   *grid = (unsigned)blocks;
   return blocks <= 0x7fffffffLL;
-}
-
-// CTAs for the kernels of a value a lane, which stride: 32 of 8 warps for each SM.
-unsigned lane_grid(int64_t rows, int64_t n) {
-  const int64_t blocks = (rows * ((n + kGroup - 1) / kGroup) + kWarps - 1) / kWarps;
-  return (unsigned)std::min<int64_t>(blocks, 148 * 32);
 }
 
 }  // namespace
@@ -237,17 +266,18 @@ int gsa_pack_e4m3(int dtype, int64_t rows, int64_t n, const void* x, int64_t x_l
   if (rows == 0 || n == 0) return GSA_OK;
   if (!x || x_ld < 0 || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  Cut c;
+  unsigned grid = 0;
+  bool fits = false;
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const T* in = static_cast<const T*>(x);
-    Cut c;
-    unsigned grid;
-    if (n % 16 == 0 && halves_ok<T>(x, x_ld) && cut(rows, n, &c, &grid))
-      pack16_kernel<T><<<grid, kThreads, 0, s>>>(c, in, x_ld, codes, c_ld, scales, s_ld);
-    else
-      pack_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, x_ld, codes, c_ld, scales, s_ld);
+    const bool halves = n % 16 == 0 && halves_ok<T>(x, x_ld);
+    if (!(fits = cut(rows, n, halves, &c, &grid))) return;
+    auto* kernel = halves ? pack16_kernel<T> : pack_kernel<T>;
+    kernel<<<grid, kThreads, 0, s>>>(c, in, x_ld, codes, c_ld, scales, s_ld);
   });
-  return launch_status();
+  return fits ? launch_status() : GSA_ERR_BAD_ARG;
 }
 
 int gsa_unpack_e4m3(int dtype, int64_t rows, int64_t n, const uint8_t* codes, int64_t c_ld, const uint8_t* scales,
@@ -256,17 +286,18 @@ int gsa_unpack_e4m3(int dtype, int64_t rows, int64_t n, const uint8_t* codes, in
   if (rows == 0 || n == 0) return GSA_OK;
   if (!x || x_ld < n || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  Cut c;
+  unsigned grid = 0;
+  bool fits = false;
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     T* out = static_cast<T*>(x);
-    Cut c;
-    unsigned grid;
-    if (n % 16 == 0 && halves_ok<T>(x, x_ld) && cut(rows, n, &c, &grid))
-      unpack16_kernel<T><<<grid, kThreads, 0, s>>>(c, codes, c_ld, scales, s_ld, out, x_ld);
-    else
-      unpack_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, codes, c_ld, scales, s_ld, out, x_ld);
+    const bool halves = n % 16 == 0 && halves_ok<T>(x, x_ld);
+    if (!(fits = cut(rows, n, halves, &c, &grid))) return;
+    auto* kernel = halves ? unpack16_kernel<T> : unpack_kernel<T>;
+    kernel<<<grid, kThreads, 0, s>>>(c, codes, c_ld, scales, s_ld, out, x_ld);
   });
-  return launch_status();
+  return fits ? launch_status() : GSA_ERR_BAD_ARG;
 }
 
 int gsa_silu_mul_pack(int dtype, int64_t rows, int64_t n, const void* gu, int64_t gu_ld, void* z, int64_t z_ld,
@@ -275,19 +306,19 @@ int gsa_silu_mul_pack(int dtype, int64_t rows, int64_t n, const void* gu, int64_
   if (rows == 0 || n == 0) return GSA_OK;
   if (!gu || gu_ld < 0 || !z || z_ld < n || !packed_ok(codes, c_ld, scales, s_ld, n)) return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  Cut c;
+  unsigned grid = 0;
+  bool fits = false;
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const T* in = static_cast<const T*>(gu);
     T* out = static_cast<T*>(z);
-    Cut c;
-    unsigned grid;
-    if (n % 16 == 0 && halves_ok<T>(gu, gu_ld) && halves_ok<T>(z, z_ld) && cut(rows, n, &c, &grid))
-      silu_mul_pack16_kernel<T><<<grid, kThreads, 0, s>>>(c, in, gu_ld, out, z_ld, codes, c_ld, scales, s_ld);
-    else
-      silu_mul_pack_kernel<T>
-          <<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, gu_ld, out, z_ld, codes, c_ld, scales, s_ld);
+    const bool halves = n % 16 == 0 && halves_ok<T>(gu, gu_ld) && halves_ok<T>(z, z_ld);
+    if (!(fits = cut(rows, n, halves, &c, &grid))) return;
+    auto* kernel = halves ? silu_mul_pack16_kernel<T> : silu_mul_pack_kernel<T>;
+    kernel<<<grid, kThreads, 0, s>>>(c, in, gu_ld, out, z_ld, codes, c_ld, scales, s_ld);
   });
-  return launch_status();
+  return fits ? launch_status() : GSA_ERR_BAD_ARG;
 }
 
 int gsa_silu_mul_packed_backward(int dtype, int64_t rows, int64_t n, const void* dz, int64_t dz_ld,
@@ -298,21 +329,20 @@ int gsa_silu_mul_packed_backward(int dtype, int64_t rows, int64_t n, const void*
   if (!dz || dz_ld < 0 || !dgu || dgu_ld < 2 * n || (z && z_ld < n) || !packed_ok(codes, c_ld, scales, s_ld, n))
     return GSA_ERR_BAD_ARG;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  Cut c;
+  unsigned grid = 0;
+  bool fits = false;
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const T* in = static_cast<const T*>(dz);
     T *out = static_cast<T*>(dgu), *again = static_cast<T*>(z);
-    Cut c;
-    unsigned grid;
-    if (n % 16 == 0 && halves_ok<T>(dz, dz_ld) && halves_ok<T>(dgu, dgu_ld) && (!z || halves_ok<T>(z, z_ld)) &&
-        cut(rows, n, &c, &grid))
-      silu_mul_bwd16_kernel<T>
-          <<<grid, kThreads, 0, s>>>(c, in, dz_ld, codes, c_ld, scales, s_ld, out, dgu_ld, again, z_ld);
-    else
-      silu_mul_bwd_kernel<T><<<lane_grid(rows, n), kThreads, 0, s>>>(rows, n, in, dz_ld, codes, c_ld, scales, s_ld,
-                                                                     out, dgu_ld, again, z_ld);
+    const bool halves = n % 16 == 0 && halves_ok<T>(dz, dz_ld) && halves_ok<T>(dgu, dgu_ld) &&
+                        (!z || halves_ok<T>(z, z_ld));
+    if (!(fits = cut(rows, n, halves, &c, &grid))) return;
+    auto* kernel = halves ? silu_mul_bwd16_kernel<T> : silu_mul_bwd_kernel<T>;
+    kernel<<<grid, kThreads, 0, s>>>(c, in, dz_ld, codes, c_ld, scales, s_ld, out, dgu_ld, again, z_ld);
   });
-  return launch_status();
+  return fits ? launch_status() : GSA_ERR_BAD_ARG;
 }
 
 }  // extern "C"

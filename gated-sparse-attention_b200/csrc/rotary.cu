@@ -20,7 +20,7 @@ namespace gsa {
 namespace {
 
 constexpr int kMaxThreads = 512;
-constexpr int kMaxTokens = 8;
+constexpr int kMaxTokens = 64;
 constexpr int kFlight = 4;        // tokens whose loads are in flight
 constexpr int kMaxAngles = 4096;  // (token, pair) entries of the shared table: 32 KB
 
@@ -45,6 +45,8 @@ struct RotaryArgs {
   float factor;
   int inverse;
   int tokens;  // per CTA
+  int beside;  // tokens that the CTA's threads take at a time
+  int items;   // places of a token
   int turn_units, units;  // of a head: units that turn, all
   int* err;
 };
@@ -167,24 +169,29 @@ template <typename T, int V, bool kInterleaved>
 __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a) {
   extern __shared__ __align__(16) float2 angles[];
   __shared__ int64_t base[kMaxTokens][4];  // element offsets of the token: q in, q out, k in, k out
+  __shared__ int64_t at_pos[kMaxTokens];
   const int half = a.rd / 2;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int n_tok = (int)min((int64_t)a.tokens, a.B * a.L - t0);
-  if ((int)threadIdx.x < n_tok) {
-    const int64_t t = t0 + threadIdx.x, b = t / a.L, l = t - b * a.L;
-    base[threadIdx.x][0] = b * a.q.ib + l * a.q.il;
-    base[threadIdx.x][1] = b * a.q.ob + l * a.q.ol;
-    base[threadIdx.x][2] = b * a.k.ib + l * a.k.il;
-    base[threadIdx.x][3] = b * a.k.ob + l * a.k.ol;
-  }
-  for (int e = threadIdx.x; e < n_tok * half; e += blockDim.x) {
-    const int tok = e / half;
+  for (int tok = threadIdx.x; tok < n_tok; tok += blockDim.x) {
     const int64_t t = t0 + tok, b = t / a.L, l = t - b * a.L;
-    angles[e] = angle_of(a, a.pos[b * a.pb + l * a.pl], e - tok * half);
+    at_pos[tok] = a.pos[b * a.pb + l * a.pl];
+    base[tok][0] = b * a.q.ib + l * a.q.il;
+    base[tok][1] = b * a.q.ob + l * a.q.ol;
+    base[tok][2] = b * a.k.ib + l * a.k.il;
+    base[tok][3] = b * a.k.ob + l * a.k.ol;
   }
   __syncthreads();
-  const int items = (a.q.heads + a.k.heads) * a.units;
-  for (int item = threadIdx.x; item < items; item += blockDim.x) {
+  for (int e = threadIdx.x; e < n_tok * half; e += blockDim.x) {
+    const int tok = e / half;
+    angles[e] = angle_of(a, at_pos[tok], e - tok * half);
+  }
+  __syncthreads();
+  // one token at a time: its places over all threads, in rounds; more: a place of one of them each
+  const int tok1 = a.beside == 1 ? 0 : threadIdx.x / a.items;
+  const int item1 = a.beside == 1 ? threadIdx.x : threadIdx.x - tok1 * a.items;
+  if (tok1 >= a.beside) return;
+  for (int item = item1; item < a.items; item += a.beside == 1 ? blockDim.x : a.items) {
     const Place p = place_of<T, V, kInterleaved>(a, item);
     const Side& s = p.is_k ? a.k : a.q;
     const T* in = static_cast<const T*>(s.in) + p.in;
@@ -192,20 +199,22 @@ __global__ void __launch_bounds__(kMaxThreads) rotary_kernel(const RotaryArgs a)
     const int64_t* at = &base[0][p.is_k ? 2 : 0];
     if (p.angle < 0 && in == out) continue;  // rotated in place: the rest is where it belongs
     // four tokens' loads before the first store, which may be to the same tensor
-    for (int tok0 = 0; tok0 < n_tok; tok0 += kFlight) {
+    for (int tok0 = tok1; tok0 < n_tok; tok0 += kFlight * a.beside) {
       Vec<T, V> x0[kFlight], x1[kFlight];
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (tok0 + j >= n_tok) break;
-        const T* x = in + at[4 * (tok0 + j)];
+        const int tok = tok0 + j * a.beside;
+        if (tok >= n_tok) break;
+        const T* x = in + at[4 * tok];
         x0[j].load(x + p.i0);
         if (p.i1 >= 0) x1[j].load(x + p.i1);
       }
 #pragma unroll
       for (int j = 0; j < kFlight; ++j) {
-        if (tok0 + j >= n_tok) break;
-        T* y = out + at[4 * (tok0 + j) + 1];
-        if (p.angle >= 0) turn<T, V, kInterleaved>(x0[j], x1[j], &angles[(tok0 + j) * half + p.angle]);
+        const int tok = tok0 + j * a.beside;
+        if (tok >= n_tok) break;
+        T* y = out + at[4 * tok + 1];
+        if (p.angle >= 0) turn<T, V, kInterleaved>(x0[j], x1[j], &angles[tok * half + p.angle]);
         x0[j].store(y + p.i0);
         if (p.i1 >= 0) x1[j].store(y + p.i1);
       }
@@ -239,13 +248,16 @@ template <typename T, int V>
 int launch_vec(RotaryArgs a, int interleaved, cudaStream_t stream) {
   a.turn_units = a.rd / 2 / V;
   a.units = a.turn_units + (a.D - a.rd + 2 * V - 1) / (2 * V);
-  const int items = (a.q.heads + a.k.heads) * a.units;
-  // threads: all places of a token in as few even rounds as fit
-  const int rounds = (items + kMaxThreads - 1) / kMaxThreads;
-  const int threads = ((items + rounds - 1) / rounds + 31) / 32 * 32;
-  // tokens a CTA: up to kMaxTokens, which spreads the angles' cost, once that leaves four CTAs for each SM
+  a.items = (a.q.heads + a.k.heads) * a.units;
+  // threads: all places of one token in as few even rounds as fit, or those of several tokens where they are few
+  a.beside = a.items < 48 ? 128 / a.items : 1;
+  const int rounds = (a.items + kMaxThreads - 1) / kMaxThreads;
+  const int threads = (a.beside > 1 ? a.beside * a.items + 31 : (a.items + rounds - 1) / rounds + 31) / 32 * 32;
+  // tokens a CTA: up to eight a thread, which spreads the angles' cost, once that leaves four CTAs for each SM
   const int64_t n = a.B * a.L;
-  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(std::min(+kMaxTokens, kMaxAngles / (a.rd / 2)), n / (4 * 148)));
+  const int most = std::min(std::min(+kMaxTokens, 8 * a.beside), kMaxAngles / (a.rd / 2));
+  a.tokens = (int)std::max<int64_t>(1, std::min<int64_t>(most, n / (4 * 148)));
+  a.beside = std::min(a.beside, a.tokens);
   const int64_t grid = (n + a.tokens - 1) / a.tokens;
   if (grid > 0x7fffffffLL) return GSA_ERR_BAD_ARG;
   const size_t smem = (size_t)a.tokens * (a.rd / 2) * sizeof(float2);

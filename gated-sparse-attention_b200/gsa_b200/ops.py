@@ -602,11 +602,11 @@ def indexer_survivors(dims: Dims, qI, kI, w, bias, scale: float, shift, k_eff: i
 # device is current.
 # ---------------------------------------------------------------------------------------------
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_CODE = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 
 
-def _run(t: torch.Tensor, name: str, *args):
-    """Call an entry point on t's device and current stream; raise GSAError on a nonzero status."""
-    dev = t.get_device()
+def _run(dev: int, name: str, *args):
+    """Call an entry point on device dev and its current stream; raise GSAError on a nonzero status."""
     fn = getattr(_lib.lib(), name)
     if dev == torch.cuda.current_device():
         st = fn(*args, _raw_stream(dev))
@@ -623,11 +623,26 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _alike(like: torch.Tensor, **ts):
-    """Every tensor given is on like's device and of its dtype."""
-    for name, t in ts.items():
-        if t is not None and (t.device != like.device or t.dtype != like.dtype):
-            raise ValueError(f"{name} is {t.dtype} on {t.device}, expected {like.dtype} on {like.device}")
+def _like(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's shape, dtype and device."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _check(like: torch.Tensor, *ts) -> int:
+    """The device index of ``like``, after checking that it is on a GPU and every tensor given is beside it and of its
+    dtype."""
+    dev, dt = like.get_device(), like.dtype
+    if dev < 0:
+        _cuda(like)
+    for t in ts:
+        if t is not None and (t.dtype is not dt or t.get_device() != dev):
+            _cuda(t)
+            raise ValueError(f"a tensor is {t.dtype} on {t.device}, expected {dt} on {like.device}")
+    return dev
+
+
+def _code(dt: torch.dtype) -> int:
+    return _CODE[dt] if dt in _CODE else dtype_code(dt)
 
 
 def _rows(t: torch.Tensor, n: int) -> torch.Tensor:
@@ -653,6 +668,22 @@ def _rotary_side(x: torch.Tensor, out: torch.Tensor) -> RotarySide:
     return RotarySide(x.data_ptr(), out.data_ptr(), x.shape[2], xb, xl, xh, ob, ol, oh)
 
 
+def _rotary_call(dev: int, q: torch.Tensor, k, q_out: torch.Tensor, k_out, positions: torch.Tensor, angles, rd: int,
+                 factor: float, interleaved: bool, inverse: bool):
+    """gsa_rotary on tensors that fit one another (as rotary checks them, and autograd its gradients)."""
+    B, L, _, D = q.shape
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    side_k = None
+    if k is not None:
+        if k.stride(3) != 1:
+            k = k.contiguous()
+        side_k = C.byref(_rotary_side(k, k_out))
+    _run(dev, "gsa_rotary", _CODE[q.dtype], B, L, D, rd, C.byref(_rotary_side(q, q_out)), side_k, positions.data_ptr(),
+         positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1), *angles, factor, interleaved,
+         inverse)
+
+
 def rotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq=None, factor: float = 1.0, interleaved: bool = False,
            inverse: bool = False, out=None, tables=None, rotary_dim=None):
     """q [B, L, H, D] and k [B, L, Hk, D] (or None) with the first ``2 * len(inv_freq)`` values of every
@@ -663,63 +694,55 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq=None, factor: f
     Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``; ``inverse`` applies the transpose (the
     backward pass).  ``out=(q_out, k_out)`` receives the results, for example K in a cache's slots; an output may
     be its input itself (rotated in place) but may not overlap an input otherwise."""
-    _cuda(q, k, positions, inv_freq)
+    dev = _check(q, k)
+    _code(q.dtype)
     if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
         raise ValueError(f"rotary takes q [B, L, H, D] and k [B, L, Hk, D], got {tuple(q.shape)} and "
                          f"{None if k is None else tuple(k.shape)}")
-    _alike(q, k=k)
     B, L, H, D = q.shape
-    cos = sin = None
+    angles = (None, None, None, 0, 0, 0)
     if tables is not None:
         cos, sin = tables
         if (cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1
-                or cos.dtype != sin.dtype or rotary_dim is None or cos.shape[1] < rotary_dim // 2):
-            raise ValueError("rotary tables are two [rows, >= rotary_dim/2] tensors of the same strides")
+                or cos.dtype != sin.dtype or rotary_dim is None or cos.shape[1] < rotary_dim // 2
+                or cos.get_device() != dev or sin.get_device() != dev):
+            raise ValueError("rotary tables are two [rows, >= rotary_dim/2] tensors of the same strides beside q")
         rd = rotary_dim
+        angles = (None, cos.data_ptr(), sin.data_ptr(), dtype_code(cos.dtype), cos.stride(0), cos.shape[0])
     else:
-        if inv_freq is None or inv_freq.dim() != 1:
-            raise ValueError("rotary takes inv_freq [rotary_dim/2]")
+        if inv_freq is None or inv_freq.dim() != 1 or inv_freq.get_device() != dev:
+            raise ValueError("rotary takes inv_freq [rotary_dim/2] beside q")
         rd = 2 * inv_freq.shape[0]
-        if inv_freq.dtype != torch.float64 or not inv_freq.is_contiguous():
+        if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
             inv_freq = inv_freq.double().contiguous()
-    for t in (positions, inv_freq, cos, sin):
-        if t is not None and t.device != q.device:
-            raise ValueError(f"rotary: a tensor on {t.device}, expected {q.device}")
+        angles = (inv_freq.data_ptr(), None, None, 0, 0, 0)
     if rd < 2 or rd > D or rd % 2 or D > 1024 or H + (0 if k is None else k.shape[2]) > 1024:
         raise ValueError(f"rotary: rotary_dim {rd} of head dim {D}, at most 1024 wide and 1024 heads")
     if positions.dim() == 1:
         positions = positions.unsqueeze(0)
     if positions.dim() != 2 or positions.shape[1] != L or positions.shape[0] not in (1, B):
         raise ValueError(f"positions {tuple(positions.shape)} for {B} sequences of {L} tokens")
-    if positions.dtype != torch.int64:
+    if positions.dtype is not torch.int64:
         if positions.dtype.is_floating_point or positions.dtype == torch.bool:
             raise ValueError("positions are integers")
         positions = positions.long()
+    if positions.get_device() != dev:
+        raise ValueError(f"positions on {positions.device}, expected {q.device}")
     if out is None:
-        q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        k_out = None if k is None else torch.empty(k.shape, device=q.device, dtype=q.dtype)
+        q_out, k_out = _like(q), None if k is None else _like(k)
     else:
         q_out, k_out = out
         for x, o in ((q, q_out), (k, k_out)):
             if (x is None) != (o is None) or (x is not None and (
-                    o.shape != x.shape or o.dtype != x.dtype or o.device != x.device
-                    or (o.shape[3] > 1 and o.stride(3) != 1) or not _separate(o))):
+                    o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev
+                    or (o.shape[3] > 1 and o.stride(3) != 1) or not (o.is_contiguous() or _separate(o)))):
                 raise ValueError("rotary: out tensors have their inputs' shape, dtype and device, contiguous values and "
                                  "no two elements in one place")
     if q.numel() == 0 and (k is None or k.numel() == 0):
         return q_out, k_out
     if H == 0 or (k is not None and k.shape[2] == 0):
         raise ValueError("rotary: a tensor without heads")
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    if k is not None and k.stride(3) != 1:
-        k = k.contiguous()
-    side_k = None if k is None else C.byref(_rotary_side(k, k_out))
-    _run(q, "gsa_rotary", dtype_code(q.dtype), B, L, D, rd, C.byref(_rotary_side(q, q_out)), side_k,
-         positions.data_ptr(), positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1),
-         _ptr(inv_freq), _ptr(cos), _ptr(sin), 0 if cos is None else dtype_code(cos.dtype),
-         0 if cos is None else cos.stride(0), 0 if cos is None else cos.shape[0], float(factor), int(interleaved),
-         int(inverse))
+    _rotary_call(dev, q, k, q_out, k_out, positions, angles, rd, factor, interleaved, inverse)
     return q_out, k_out
 
 
@@ -733,13 +756,13 @@ class PackedActivation:
     __slots__ = ("data", "shape", "dtype")
 
     def __init__(self, data: torch.Tensor, shape, dtype: torch.dtype):
-        self.data, self.shape, self.dtype = data, torch.Size(shape), dtype
+        self.data, self.shape, self.dtype = data, tuple(shape), dtype
 
     @classmethod
     def empty(cls, shape, dtype: torch.dtype, device) -> "PackedActivation":
         n = shape[-1]
         rows = math.prod(shape[:-1])
-        return cls(torch.empty(rows * ((n + 15) // 16 * 16 + (n + 31) // 32), device=device, dtype=torch.uint8), shape,
+        return cls(torch.empty(rows * ((n + 15) // 16 * 16 + (n + 31) // 32), dtype=torch.uint8, device=device), shape,
                    dtype)
 
     @property
@@ -783,58 +806,58 @@ class PackedActivation:
 
 def pack_e4m3(x: torch.Tensor) -> PackedActivation:
     """x [..., n] in 8 bits."""
-    _cuda(x)
+    dev = _check(x)
     if x.dim() == 0:
         raise ValueError("pack_e4m3 takes a tensor with a last dimension")
-    code = dtype_code(x.dtype)
+    code = _code(x.dtype)
     n = x.shape[-1]
     p = PackedActivation.empty(x.shape, x.dtype, x.device)
     if x.numel():
         x2 = _rows(x, n)
-        _run(x, "gsa_pack_e4m3", code, x2.shape[0], n, x2.data_ptr(), x2.stride(0), *p._args())
+        _run(dev, "gsa_pack_e4m3", code, x2.shape[0], n, x2.data_ptr(), x2.stride(0), *p._args())
     return p
 
 
 def unpack_e4m3(p: PackedActivation, dtype=None) -> torch.Tensor:
     """The values of a packed tensor, in its dtype or the given one."""
-    x = torch.empty(p.shape, device=p.data.device, dtype=dtype or p.dtype)
-    code = dtype_code(x.dtype)
+    x = p.data.new_empty(p.shape, dtype=dtype or p.dtype)
+    code = _code(x.dtype)
     if x.numel():
         n = p.shape[-1]
-        _run(x, "gsa_unpack_e4m3", code, x.numel() // n, n, *p._args(), x.data_ptr(), n)
+        _run(_check(x), "gsa_unpack_e4m3", code, x.numel() // n, n, *p._args(), x.data_ptr(), n)
     return x
 
 
 def silu_mul_packed(gu: torch.Tensor):
     """(z, packed): z = silu(g) * u of gu [..., 2n] = (g, u), and (g, u) packed as [..., 2, n]."""
-    _cuda(gu)
+    dev = _check(gu)
     if gu.dim() == 0 or gu.shape[-1] % 2:
         raise ValueError(f"silu_mul_packed takes [..., 2n], got {tuple(gu.shape)}")
-    code = dtype_code(gu.dtype)
+    code = _code(gu.dtype)
     n = gu.shape[-1] // 2
     lead = gu.shape[:-1]
-    z = torch.empty(*lead, n, device=gu.device, dtype=gu.dtype)
+    z = gu.new_empty((*lead, n))
     p = PackedActivation.empty((*lead, 2, n), gu.dtype, gu.device)
     if z.numel():
         g2 = _rows(gu, 2 * n)
-        _run(gu, "gsa_silu_mul_pack", code, g2.shape[0], n, g2.data_ptr(), g2.stride(0), z.data_ptr(), n, *p._args())
+        _run(dev, "gsa_silu_mul_pack", code, g2.shape[0], n, g2.data_ptr(), g2.stride(0), z.data_ptr(), n, *p._args())
     return z, p
 
 
 def silu_mul_packed_backward(dz: torch.Tensor, packed: PackedActivation, want_z: bool = False):
     """(dgu [..., 2n], z or None) of silu_mul_packed from dz [..., n] and the packed (g, u); z is that of the packed
     values, for the weight gradient of the product that reads it."""
-    _cuda(dz)
+    dev = _check(dz)
     if len(packed.shape) < 2 or packed.shape[-2] != 2 or dz.shape != packed.shape[:-2] + packed.shape[-1:]:
         raise ValueError(f"dz {tuple(dz.shape)} for packed {tuple(packed.shape)}")
-    if dz.dtype != packed.dtype or dz.device != packed.data.device:
+    if dz.dtype is not packed.dtype or packed.data.get_device() != dev:
         raise ValueError(f"dz is {dz.dtype} on {dz.device}, packed {packed.dtype} on {packed.data.device}")
     n = packed.shape[-1]
-    dgu = torch.empty(*dz.shape[:-1], 2 * n, device=dz.device, dtype=dz.dtype)
-    z = torch.empty(dz.shape, device=dz.device, dtype=dz.dtype) if want_z else None
+    dgu = dz.new_empty((*dz.shape[:-1], 2 * n))
+    z = _like(dz) if want_z else None
     if dz.numel():
         d2 = _rows(dz, n)
-        _run(dz, "gsa_silu_mul_packed_backward", dtype_code(dz.dtype), d2.shape[0], n, d2.data_ptr(), d2.stride(0),
+        _run(dev, "gsa_silu_mul_packed_backward", _code(dz.dtype), d2.shape[0], n, d2.data_ptr(), d2.stride(0),
              *packed._args(), dgu.data_ptr(), 2 * n, _ptr(z), n)
     return dgu, z
 
@@ -842,23 +865,22 @@ def silu_mul_packed_backward(dz: torch.Tensor, packed: PackedActivation, want_z:
 def add_rmsnorm_packed(x: torch.Tensor, a, weight: torch.Tensor, eps: float):
     """(h, y, packed, rstd): h = x + a (None when a is None: h is x), y = RMSNorm(h) * weight over the last
     dimension, h packed, and rstd [...] fp32 -- what rmsnorm_packed_backward needs."""
-    _cuda(x, a, weight)
+    dev = _check(x, a, weight)
     if x.dim() == 0 or x.shape[-1] == 0 or weight.shape != x.shape[-1:] or (a is not None and a.shape != x.shape):
         raise ValueError(f"add_rmsnorm_packed: x {tuple(x.shape)}, a {None if a is None else tuple(a.shape)}, weight "
                          f"{tuple(weight.shape)}")
-    _alike(x, a=a, weight=weight)
-    code = dtype_code(x.dtype)
+    code = _code(x.dtype)
     d = x.shape[-1]
-    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if a is not None else None
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    rstd = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    h = _like(x) if a is not None else None
+    y = _like(x)
+    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
     p = PackedActivation.empty(x.shape, x.dtype, x.device)
     if x.numel():
         x2 = _rows(x, d)
         a2 = None if a is None else _rows(a, d)
         w = weight.contiguous()
-        _run(x, "gsa_add_rmsnorm_pack", code, x2.shape[0], d, x2.data_ptr(), x2.stride(0), _ptr(a2),
-             0 if a2 is None else a2.stride(0), w.data_ptr(), float(eps), _ptr(h), d, y.data_ptr(), d,
+        _run(dev, "gsa_add_rmsnorm_pack", code, x2.shape[0], d, x2.data_ptr(), x2.stride(0), _ptr(a2),
+             0 if a2 is None else a2.stride(0), w.data_ptr(), eps, _ptr(h), d, y.data_ptr(), d,
              *p._args(), rstd.data_ptr())
     return h, y, p, rstd
 
@@ -868,30 +890,29 @@ def rmsnorm_packed_backward(dy: torch.Tensor, packed: PackedActivation, rstd: to
     """(dx, dw or None, y or None) of y = RMSNorm(h) * weight from dy, the packed h and rstd; ``dh`` (the gradient
     that reaches h past the norm) is added to dx.  y is that of the packed h, for the weight gradients of the
     products that read it."""
-    _cuda(dy, rstd, weight, dh)
+    dev = _check(dy, weight, dh)
     if dy.shape != packed.shape or weight.shape != dy.shape[-1:] or (dh is not None and dh.shape != dy.shape) \
-            or rstd.shape != dy.shape[:-1] or rstd.dtype != torch.float32 or dy.shape[-1] == 0:
+            or rstd.shape != dy.shape[:-1] or rstd.dtype is not torch.float32 or dy.shape[-1] == 0:
         raise ValueError(f"rmsnorm_packed_backward: dy {tuple(dy.shape)}, packed {tuple(packed.shape)}, weight "
                          f"{tuple(weight.shape)}, rstd {tuple(rstd.shape)}")
-    _alike(dy, weight=weight, dh=dh)
-    if packed.dtype != dy.dtype or packed.data.device != dy.device or rstd.device != dy.device:
+    if packed.dtype is not dy.dtype or packed.data.get_device() != dev or rstd.get_device() != dev:
         raise ValueError(f"dy is {dy.dtype} on {dy.device}, packed {packed.dtype} on {packed.data.device}")
     d = dy.shape[-1]
     rows = dy.numel() // d
-    dx = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype)
-    y = torch.empty(dy.shape, device=dy.device, dtype=dy.dtype) if want_y else None
+    dx = _like(dy)
+    y = _like(dy) if want_y else None
     if rows == 0:
-        return dx, (torch.zeros(d, device=dy.device, dtype=dy.dtype) if want_dw else None), y
+        return dx, (dy.new_zeros(d) if want_dw else None), y
     dw = ws = None
     nbytes = 0
     if want_dw:
-        dw = torch.empty(d, device=dy.device, dtype=dy.dtype)
+        dw = dy.new_empty(d)
         nbytes = _lib.lib().gsa_rmsnorm_packed_workspace_size(rows, d)
-        ws = torch.empty(nbytes, device=dy.device, dtype=torch.uint8)
+        ws = rstd.new_empty(nbytes // 4)
     d2 = _rows(dy, d)
     h2 = None if dh is None else _rows(dh, d)
     w, rstd = weight.contiguous(), rstd.contiguous()
-    _run(dy, "gsa_rmsnorm_packed_backward", dtype_code(dy.dtype), rows, d, d2.data_ptr(), d2.stride(0), _ptr(h2),
+    _run(dev, "gsa_rmsnorm_packed_backward", _code(dy.dtype), rows, d, d2.data_ptr(), d2.stride(0), _ptr(h2),
          0 if h2 is None else h2.stride(0), w.data_ptr(), *packed._args(), rstd.data_ptr(), dx.data_ptr(), d, _ptr(y), d, _ptr(dw), _ptr(ws), nbytes)
     return dx, dw, y
 
@@ -900,24 +921,25 @@ def next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: in
     """(loss, grad or None): mean cross entropy of labels[:, t + 1] under logits[:, t] ([B, L, V]), fp32, and its
     gradient in the logits' dtype.  Labels equal to ignore_index do not count; without any that count the loss is NaN
     and the gradient 0."""
-    _cuda(logits, labels)
+    dev = _check(logits)
     if logits.dim() != 3 or logits.shape[2] == 0 or labels.shape != logits.shape[:2]:
         raise ValueError(f"next_token_loss takes logits [B, L, V] and labels [B, L], got {tuple(logits.shape)} and "
                          f"{tuple(labels.shape)}")
-    if labels.device != logits.device:
+    if labels.get_device() != dev:
+        _cuda(labels)
         raise ValueError(f"labels on {labels.device}, logits on {logits.device}")
-    if labels.dtype != torch.int64:
+    if labels.dtype is not torch.int64:
         if labels.dtype.is_floating_point or labels.dtype == torch.bool:
             raise ValueError("labels are integers")
         labels = labels.long()
-    code = dtype_code(logits.dtype)
+    code = _code(logits.dtype)
     B, L, V = logits.shape
     x = logits if V == 1 or logits.stride(2) == 1 else logits.contiguous()
-    loss = torch.empty((), device=logits.device, dtype=torch.float32)
+    loss = logits.new_empty((), dtype=torch.float32)
     nbytes = _lib.lib().gsa_next_token_loss_workspace_size()
-    ws = torch.empty(nbytes, device=logits.device, dtype=torch.uint8)
-    grad = torch.empty(B, L, V, device=logits.device, dtype=logits.dtype) if want_grad else None
-    _run(logits, "gsa_next_token_loss", code, B, L, V, x.data_ptr(), x.stride(0), x.stride(1), labels.data_ptr(),
+    ws = logits.new_empty(nbytes, dtype=torch.uint8)
+    grad = _like(logits) if want_grad else None
+    _run(dev, "gsa_next_token_loss", code, B, L, V, x.data_ptr(), x.stride(0), x.stride(1), labels.data_ptr(),
          labels.stride(0), labels.stride(1), int(ignore_index), loss.data_ptr(), _ptr(grad), L * V, V,
          ws.data_ptr(), nbytes)
     return loss, grad
@@ -925,9 +947,9 @@ def next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: in
 
 def scale_(x: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
     """x *= factor in place, for a contiguous x and a one-element fp32 tensor factor; a factor of 1 leaves x unread."""
-    _cuda(x, factor)
-    if not x.is_contiguous() or factor.numel() != 1 or factor.dtype != torch.float32 or factor.device != x.device:
+    dev = _check(x)
+    if not x.is_contiguous() or factor.numel() != 1 or factor.dtype is not torch.float32 or factor.get_device() != dev:
         raise ValueError("scale_ takes a contiguous tensor and a one-element fp32 factor on its device")
     if x.numel():
-        _run(x, "gsa_scale", dtype_code(x.dtype), x.numel(), x.data_ptr(), factor.data_ptr())
+        _run(dev, "gsa_scale", _code(x.dtype), x.numel(), x.data_ptr(), factor.data_ptr())
     return x

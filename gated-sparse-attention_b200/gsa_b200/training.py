@@ -95,23 +95,30 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[Dict[s
 class _Rotary(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, positions, inv_freq, factor, interleaved):
+        out = ops.rotary(q, k, positions, inv_freq, factor, interleaved)  # refuses what does not fit
+        if positions.dim() == 1:
+            positions = positions.unsqueeze(0)
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions, inv_freq)
+        ctx.save_for_backward(positions.long(), inv_freq.double().contiguous())
         ctx.how = (factor, interleaved)
-        return ops.rotary(q, k, positions, inv_freq, factor, interleaved)
+        return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq, dk):
         positions, inv_freq = ctx.saved_tensors
         factor, interleaved = ctx.how
-        dq = dq if ctx.needs_input_grad[0] else None
-        dk = dk if ctx.needs_input_grad[1] else None
-        if dq is not None:
-            dq, dk = ops.rotary(dq, dk, positions, inv_freq, factor, interleaved, inverse=True)
-        elif dk is not None:
-            dk = ops.rotary(dk, None, positions, inv_freq, factor, interleaved, inverse=True)[0]
-        return dq, dk, None, None, None, None
+        need = ctx.needs_input_grad
+        grads = [dq if need[0] else None, dk if need[1] else None]
+        given = [g for g in grads if g is not None]
+        if given and given[0].numel():
+            q, k = given[0], given[1] if len(given) > 1 else None
+            q_out, k_out = ops._like(q), None if k is None else ops._like(k)
+            ops._rotary_call(q.get_device(), q, k, q_out, k_out, positions, (inv_freq.data_ptr(), None, None, 0, 0, 0),
+                             2 * inv_freq.shape[0], factor, interleaved, True)
+            outs = iter((q_out, k_out))
+            grads = [None if g is None else next(outs) for g in grads]
+        return grads[0], grads[1], None, None, None, None
 
 
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
@@ -251,7 +258,9 @@ class _NextTokenLoss(torch.autograd.Function):
         if grad is None:
             raise RuntimeError("fused_next_token_loss: its gradient was handed out by an earlier backward pass; call it "
                                "again for another")
-        return ops.scale_(grad, d_loss), None, None
+        ops._run(grad.get_device(), "gsa_scale", ops._CODE[grad.dtype], grad.numel(), grad.data_ptr(),
+                 d_loss.data_ptr())
+        return grad, None, None
 
 
 def fused_next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
