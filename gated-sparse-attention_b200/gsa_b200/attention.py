@@ -568,7 +568,8 @@ def _act_grad(logits: torch.Tensor, act: str) -> torch.Tensor:
 
 def _rope_backward(dy: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor) -> torch.Tensor:
     """Transpose of y = x cos + rotate_half(x) sin (rope.py:151-185): rotate_half maps (x1, x2) to
-    (-x2, x1), its transpose maps (y1, y2) to (y2, -y1).  dy [T, heads, D] fp32, cos/sin [T, D]."""
+    (-x2, x1), its transpose maps (y1, y2) to (y2, -y1).  dy [T, heads, D] fp32, cos/sin [T, D].  The torch
+    form of ops.rotary(inverse=True), which gives the same bits."""
     c, s_ = cos.float().unsqueeze(1), sin.float().unsqueeze(1)
     ys = dy * s_
     h = dy.shape[-1] // 2
@@ -619,14 +620,13 @@ class _GSATrain(torch.autograd.Function):
                 dO, d_g1 = d_gated, None
             dq, dk, dv = ops.sparse_sdpa_backward(sv["dims"], sv["q"], sv["k"], sv["v"], sv["sel"], sv["cnt"],
                                                   sv["O"], dO.view(B, L, H, D), sv["lse"], layer.scale)
-            pos = sv["positions"].reshape(-1)
-            cos, sin = layer.rotary_emb.cos_cached[pos], layer.rotary_emb.sin_cached[pos]
-            dq_raw = _rope_backward(dq.view(T, H, D), cos, sin)
-            dk_raw = _rope_backward(dk.reshape(T, Hk, D), cos, sin)
             dv = dv.reshape(T, Hk * D)
             d_proj = torch.zeros(T, W.shape[0], device=x.device, dtype=torch.float32)
-            d_proj[:, lay.q:lay.q + H * D] = dq_raw.reshape(T, H * D)
-            d_proj[:, lay.k:lay.k + Hk * D] = dk_raw.reshape(T, Hk * D)
+            # the gradients of q and k, turned back by their positions, straight into their columns
+            ops.rotary(dq, dk, sv["positions"].reshape(B, L), inverse=True, rotary_dim=D,
+                       tables=(layer.rotary_emb.cos_cached, layer.rotary_emb.sin_cached),
+                       out=(d_proj[:, lay.q:lay.q + H * D].view(B, L, H, D),
+                            d_proj[:, lay.k:lay.k + Hk * D].view(B, L, Hk, D)))
             if lay.g2 >= 0:
                 act = layer.value_gate.activation
                 v_raw = proj[:, lay.v:lay.v + Hk * D].float()

@@ -17,7 +17,9 @@ before construction gives the reference's weights and state dicts load either wa
 Without autograd the decoder layer runs: the fused residual-add + RMSNorm kernel, the attention
 layer (its own kernels), and a SwiGLU MLP of one GEMM over the concatenated gate/up weights, the
 silu-product kernel and the down GEMM (cuBLAS).  Under autograd the norm and MLP use the
-reference's torch formulas (differentiable) around the attention's autograd function.
+reference's torch formulas (differentiable) around the attention's autograd function; with
+``enable_packed_training`` they keep their activations in 8 bits instead, and the loss forms its
+gradient in one pass over the logits (training.py).
 """
 
 from __future__ import annotations
@@ -29,7 +31,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from . import ops
+from . import ops, training
 from .attention import GatedSparseAttention
 from .config import GSAConfig
 
@@ -102,11 +104,24 @@ class GSADecoderLayer(nn.Module):
         self.self_attn = GatedSparseAttention(config)
         self.post_attention_layernorm = RMSNorm(config.d_model, eps=config.norm_eps)
         self.mlp = GSAMlp(config)
+        self.packed_training = False  # under autograd: norm and MLP activations kept in 8 bits
+
+    def _forward_packed(self, hidden_states, **attn):
+        n1, n2, mlp = self.input_layernorm, self.post_attention_layernorm, self.mlp
+        _, normed = training.packed_add_rmsnorm(hidden_states, None, n1.weight, n1.eps)
+        attn_output, present_key_value, attn_weights = self.self_attn(normed, **attn)
+        out = training.packed_mlp_block(hidden_states, attn_output, n2.weight, mlp.gate_proj.weight,
+                                        mlp.up_proj.weight, mlp.down_proj.weight, n2.eps)
+        return out, present_key_value, attn_weights
 
     def forward(self, hidden_states: torch.Tensor, positions: Optional[torch.Tensor] = None,
                 attention_mask: Optional[torch.Tensor] = None,
                 past_key_value: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                 use_cache: bool = False, output_attentions: bool = False):
+        if self.packed_training and not _fused(hidden_states, *self.parameters()):
+            return self._forward_packed(hidden_states, positions=positions, attention_mask=attention_mask,
+                                        past_key_value=past_key_value, use_cache=use_cache,
+                                        output_attentions=output_attentions)
         residual = hidden_states
         hidden_states = self.input_layernorm(hidden_states)
         attn_output, present_key_value, attn_weights = self.self_attn(
@@ -163,7 +178,16 @@ class GSALlamaModel(nn.Module):
         self.layers = nn.ModuleList([GSADecoderLayer(config, layer_idx=i) for i in range(config.n_layers)])
         self.norm = RMSNorm(config.d_model, eps=config.norm_eps)
         self.gradient_checkpointing = False
+        self.packed_training = False
         self._init_weights()
+
+    def enable_packed_training(self, enabled: bool = True):
+        """Under autograd, keep the norms' and the MLPs' activations in 8 bits for the backward pass: 33/32 bytes a
+        value of h and of the MLP's (g, u), where the torch formulas keep some ten copies in 16 and 32 bits.  The
+        forward pass is not quantised; gradients are those at the kept values (within 2^-4 of the values each)."""
+        self.packed_training = bool(enabled)
+        for layer in self.layers:
+            layer.packed_training = bool(enabled)
 
     def _init_weights(self):
         nn.init.normal_(self.embed_tokens.weight, std=self.config.initializer_range)
@@ -198,7 +222,10 @@ class GSALlamaModel(nn.Module):
                                                 output_attentions)
             presents.append(present)
             weights.append(attn)
-        h = self.norm(h)
+        if self.packed_training and not _fused(h, self.norm.weight):
+            h = training.packed_add_rmsnorm(h, None, self.norm.weight, self.norm.eps)[1]
+        else:
+            h = self.norm(h)
         seen.append(h)
         return GSAModelOutput(last_hidden_state=h,
                               past_key_values=tuple(presents) if use_cache else None,
@@ -283,9 +310,15 @@ class GSALlamaForCausalLM(nn.Module):
                           past_key_values=past_key_values, use_cache=use_cache,
                           output_attentions=output_attentions, output_hidden_states=output_hidden_states)
         logits = self.lm_head(base.last_hidden_state)
-        return GSACausalLMOutput(loss=None if labels is None else next_token_loss(logits, labels), logits=logits,
+        loss_of = training.fused_next_token_loss if self.model.packed_training else next_token_loss
+        return GSACausalLMOutput(loss=None if labels is None else loss_of(logits, labels), logits=logits,
                                  past_key_values=base.past_key_values, hidden_states=base.hidden_states,
                                  attentions=base.attentions)
+
+    def enable_packed_training(self, enabled: bool = True):
+        """GSALlamaModel.enable_packed_training, and the loss in fp32 with its gradient formed in the same pass over the
+        logits (fused_next_token_loss) instead of next_token_loss."""
+        self.model.enable_packed_training(enabled)
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, max_new_tokens: int = 100, temperature: float = 1.0,

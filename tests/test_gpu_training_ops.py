@@ -673,3 +673,117 @@ def test_captured_training_step(cuda_ok):
         g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+# -- together -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,d,n", [(5, 48, 33), (64, 256, 512)])
+def test_packed_mlp_block(cuda_ok, dtype, rows, d, n):
+    """The block's output and every gradient against the 64-bit formulas at the values that the kernels keep (the packed
+    tensors of the same calls): matrix products of k terms lose up to k U and a half step of each operand in between."""
+    import gsa_b200 as gsa
+
+    x, a = _randn(1, rows, d, dtype=dtype), _randn(2, rows, d, dtype=dtype)
+    w = (1 + 0.1 * _randn(3, d)).to(dtype)
+    wg, wu, wd = (_randn(4 + i, *s, dtype=dtype, scale=s[1] ** -0.5) for i, s in enumerate(((n, d), (n, d), (d, n))))
+    dout = _randn(8, rows, d, dtype=dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, a, w, wg, wu, wd)]
+    out = gsa.packed_mlp_block(*leaves, 1e-5)
+    grads = torch.autograd.grad(out, leaves, dout)
+    # the same kernels by hand, for what they keep
+    h, y, ph, rstd = gsa.ops.add_rmsnorm_packed(x, a, w, 1e-5)
+    gu = torch.empty(rows, 2 * n, device=DEV, dtype=dtype)
+    torch.mm(y, wg.t(), out=gu[:, :n])
+    torch.mm(y, wu.t(), out=gu[:, n:])
+    z, pgu = gsa.ops.silu_mul_packed(gu)
+    D = lambda t: t.double()
+    hh, guh, r = D(ph.unpack(torch.float32)), D(pgu.unpack(torch.float32)), D(rstd).unsqueeze(-1)
+    g, u = guh[:, 0], guh[:, 1]
+    sig = torch.sigmoid(g)
+    yk, zk = hh * r * D(w), g * sig * u
+    dz = D(dout) @ D(wd)
+    dg, du = dz * u * sig * (1 + g * (1 - sig)), dz * g * sig
+    dy = dg @ D(wg) + du @ D(wu)
+    xh = hh * r
+    dx = r * (dy * D(w) - xh * (dy * D(w) * xh).mean(-1, keepdim=True)) + D(dout)
+    want = [dx, dx, (dy * xh).sum(0), dg.t() @ yk, du.t() @ yk, D(dout).t() @ zk]
+    # sums of absolute values: what each result is made of; every rounded operand in between is off by half a step
+    e = _half_step(dtype)
+    ab = torch.abs
+    mdz = ab(D(dout)) @ ab(D(wd))
+    mdg, mdu = mdz * ab(u) * sig * (1 + ab(g)), mdz * ab(g) * sig
+    mdy = mdg @ ab(D(wg)) + mdu @ ab(D(wu))
+    mdx = r * (mdy * ab(D(w)) + ab(xh) * (mdy * ab(D(w) * xh)).mean(-1, keepdim=True)) + ab(D(dout))
+    made = [mdx, mdx, (mdy * ab(xh)).sum(0), mdg.t() @ ab(yk), mdu.t() @ ab(yk), ab(D(dout)).t() @ ab(zk)]
+    for name, got, ref, m in zip(("x", "a", "w", "gate", "up", "down"), grads, want, made):
+        _near(got, ref, m * (6 * e + (n + d + rows + 64) * U), name)
+    # the down product is the matrix library's, which may round the product, and partial sums of it, to the type before h
+    # is added (torch allows bf16 reductions by default): a half step of the terms' sizes for each of the two
+    ref, made = D(h) + D(z) @ D(wd).t(), ab(D(z)) @ ab(D(wd)).t()
+    _near(out.detach(), ref, (ab(D(h)) + made) * (n + 8) * U + 2 * e * made, "out")
+    # frozen parts get no gradient, the others the same
+    some = [t.clone().requires_grad_(i in (0, 3)) for i, t in enumerate((x, a, w, wg, wu, wd))]
+    got = torch.autograd.grad(gsa.packed_mlp_block(*some, 1e-5), (some[0], some[3]), dout)
+    assert torch.equal(got[0], grads[0]) and torch.equal(got[1], grads[3])
+
+
+def _lm(dtype, layers=2):
+    from gsa_b200 import GSAConfig, GSALlamaForCausalLM
+
+    cfg = GSAConfig(d_model=256, n_heads=4, n_kv_heads=2, d_indexer=32, n_indexer_heads=4, k_base=24, k_min=8, k_max=48,
+                    n_layers=layers, d_ffn=512, vocab_size=384, max_position_embeddings=512)
+    torch.manual_seed(0)
+    return GSALlamaForCausalLM(cfg).to(DEV).to(dtype).train()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_causal_lm_packed_training_step(cuda_ok, dtype):
+    """The model's training step with packed activations and the fused loss: the loss is the torch one, every trainable
+    parameter gets a gradient near the unpacked step's.  Each kept value is within 2^-4 of its value and a term of a
+    gradient has at most four of them, so gradients differ by less than 4 / 16 in norm."""
+    m = _lm(dtype)
+    ids = torch.randint(0, 384, (2, 64), generator=torch.Generator().manual_seed(2)).to(DEV)
+    plain = m(ids, labels=ids)
+    plain.loss.backward()
+    ref = {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}
+    m.zero_grad(set_to_none=True)
+    m.enable_packed_training()
+    out = m(ids, labels=ids)
+    out.loss.backward()
+    assert out.loss.dtype == torch.float32
+    exact = torch.nn.functional.cross_entropy(out.logits.double()[:, :-1].reshape(-1, 384), ids[:, 1:].reshape(-1))
+    assert abs(float(out.loss.detach()) - float(exact.detach())) < 1e-5 * float(exact.detach())
+    for name, p in m.named_parameters():
+        if ".indexer." in name:
+            assert p.grad is None, name
+            continue
+        assert p.grad is not None and p.grad.dtype == dtype and bool(torch.isfinite(p.grad).all()), name
+        off = float((p.grad.double() - ref[name].double()).norm() / ref[name].double().norm())
+        assert off < 0.25, (name, off)
+    # without autograd, and switched off again, the model is what it was
+    with torch.no_grad():
+        a = m(ids).logits
+    m.enable_packed_training(False)
+    with torch.no_grad():
+        assert torch.equal(m(ids).logits, a)
+    m.zero_grad(set_to_none=True)
+    again = m(ids, labels=ids)
+    assert torch.equal(again.loss, plain.loss)
+
+
+def test_packed_training_holds_less(cuda_ok):
+    """Memory that the graph of a step keeps (allocated after the forward pass, above the weights)."""
+    m = _lm(torch.bfloat16, layers=4)
+    ids = torch.randint(0, 384, (4, 512), generator=torch.Generator().manual_seed(2)).to(DEV)
+    kept = []
+    for packed in (False, True):
+        m.enable_packed_training(packed)
+        m(ids)  # caches of the layers
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = m.model(ids).last_hidden_state
+        torch.cuda.synchronize()
+        kept.append(torch.cuda.memory_allocated() - before)
+        del out
+    # what the layers keep beside the attention goes from 16- and 32-bit copies to 33/32 bytes a value
+    assert kept[1] < 0.75 * kept[0], kept
