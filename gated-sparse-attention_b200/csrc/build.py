@@ -1,8 +1,8 @@
-"""Build libgsa_b200.so (sm_100a) in-tree with nvcc.
+"""Build libgsa_b200.so (sm_100a) in-tree with nvcc, and the torch binding of the training-step operators with g++.
 
 Each .cu file is compiled to an object in parallel, then linked into
 ``gated-sparse-attention_b200/gsa_b200/libgsa_b200.so`` next to the Python package that loads
-it.  Run directly (``python gated-sparse-attention_b200/csrc/build.py``) or through
+it; ``torch_ops.cpp`` becomes ``_native.so`` beside it.  Run directly (``python gated-sparse-attention_b200/csrc/build.py``) or through
 ``__graft_entry__.build()``.
 """
 
@@ -21,6 +21,8 @@ REPO = PKG_ROOT.parent
 OUT_DIR = PKG_ROOT / "gsa_b200"
 LIB = OUT_DIR / "libgsa_b200.so"
 OBJ_DIR = PKG_ROOT / "_build"
+NATIVE_SRC = CSRC / "torch_ops.cpp"
+NATIVE = OUT_DIR / "_native.so"
 
 SOURCES = ["abi.cu", "proj_epilogue.cu", "indexer_simt.cu", "indexer_tc.cu", "indexer_decode.cu", "topk.cu",
            "sparse_sdpa.cu", "sparse_sdpa_bwd.cu", "select_static.cu", "decoder.cu", "sdpa_probs.cu", "selftest.cu",
@@ -51,6 +53,24 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool, ptxas_v: bool) -> s
     return res.stderr if (verbose or ptxas_v) else ""
 
 
+def _compile_native() -> None:
+    """_native.so: torch_ops.cpp against the installed torch's headers and libraries."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    inc = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", Path(_nvcc()).parent.parent / "include",
+           Path("/usr/local/cuda/include"), Path(sysconfig.get_paths()["include"]), REPO / "include"]
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-DTORCH_EXTENSION_NAME=_native",
+           *[f"-I{p}" for p in inc], str(NATIVE_SRC), "-o", str(NATIVE), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda",
+           "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {NATIVE_SRC.name}:\n{res.stdout}\n{res.stderr}")
+
+
 def build(verbose: bool = False, ptxas_v: bool = False, force: bool = False) -> Path:
     nvcc = _nvcc()
     OBJ_DIR.mkdir(exist_ok=True)
@@ -59,6 +79,10 @@ def build(verbose: bool = False, ptxas_v: bool = False, force: bool = False) -> 
     newest_header = max(h.stat().st_mtime for h in headers)
     jobs = []
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
+        native = None
+        abi_time = max(NATIVE_SRC.stat().st_mtime, (REPO / "include" / "gsa_b200.h").stat().st_mtime)
+        if force or not NATIVE.exists() or NATIVE.stat().st_mtime < abi_time:
+            native = ex.submit(_compile_native)
         for src in srcs:
             obj = OBJ_DIR / (src.stem + ".o")
             stale = (force or not obj.exists() or obj.stat().st_mtime < src.stat().st_mtime
@@ -69,6 +93,8 @@ def build(verbose: bool = False, ptxas_v: bool = False, force: bool = False) -> 
             log = fut.result()
             if log:
                 print(f"--- {src.name}\n{log}", file=sys.stderr)
+        if native is not None:
+            native.result()
     objs = [str(OBJ_DIR / (s.stem + ".o")) for s in srcs]
     if jobs or not LIB.exists():
         cmd = [nvcc, *ARCH, "-shared", "-o", str(LIB), *objs, "-lcudart", "-lcuda"]

@@ -146,6 +146,31 @@ def lib():
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The torch binding of the training-step operators (_native.so), its entry points taken from the loaded library;
+    raises if either is missing."""
+    global _native
+    if _native is None:
+        handle = lib()
+        with _lock:
+            if _native is None:
+                try:
+                    from . import _native as mod
+                except ImportError as e:
+                    raise RuntimeError(
+                        f"GSA torch binding not found or not loadable beside {LIB_PATH.name}; build it with "
+                        "`python gated-sparse-attention_b200/csrc/build.py`") from e
+                names = ("gsa_rotary", "gsa_pack_e4m3", "gsa_unpack_e4m3", "gsa_silu_mul_pack", "gsa_silu_mul_packed_backward",
+                         "gsa_add_rmsnorm_pack", "gsa_rmsnorm_packed_workspace_size", "gsa_rmsnorm_packed_backward",
+                         "gsa_next_token_loss", "gsa_next_token_loss_workspace_size", "gsa_scale")
+                mod.bind({n: C.cast(getattr(handle, n), C.c_void_p).value for n in names}, GSAError)
+                _native = mod
+    return _native
+
+
 def call(name: str, *args) -> int:
     """Call an entry point and raise GSAError on a nonzero status."""
     st = getattr(lib(), name)(*args)

@@ -14,7 +14,7 @@ import os
 import torch
 
 from . import _lib
-from ._lib import ACT, DTYPE_BF16, DTYPE_F32, Dims, ProjLayout, RotarySide, TopkParams
+from ._lib import ACT, DTYPE_BF16, DTYPE_F32, Dims, ProjLayout, TopkParams
 
 DEBUG = os.environ.get("GSA_DEBUG", "0") == "1"
 # number of (indexer, top-k) chunk launches of the last indexer_select call
@@ -598,152 +598,22 @@ def indexer_survivors(dims: Dims, qI, kI, w, bias, scale: float, shift, k_eff: i
 
 # ---------------------------------------------------------------------------------------------
 # Training-step operators around the attention: rotary positions, activations kept in 8 bits, the
-# next-token loss.  These run on their tensors' device and that device's current stream, whichever
-# device is current.
+# next-token loss.  Their checks, outputs and calls are in csrc/torch_ops.cpp; they run on their tensors'
+# device and that device's current stream, whichever device is current.
 # ---------------------------------------------------------------------------------------------
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_CODE = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
-
-
-def _run(dev: int, name: str, *args):
-    """Call an entry point on device dev and its current stream; raise GSAError on a nonzero status."""
-    fn = getattr(_lib.lib(), name)
-    if dev == torch.cuda.current_device():
-        st = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, _raw_stream(dev))
-    if st:
-        raise _lib.GSAError(name, st)
-    if DEBUG:
-        _after(name)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _like(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised contiguous tensor of t's shape, dtype and device."""
-    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
-
-
-def _check(like: torch.Tensor, *ts) -> int:
-    """The device index of ``like``, after checking that it is on a GPU and every tensor given is beside it and of its
-    dtype."""
-    dev, dt = like.get_device(), like.dtype
-    if dev < 0:
-        _cuda(like)
-    for t in ts:
-        if t is not None and (t.dtype is not dt or t.get_device() != dev):
-            _cuda(t)
-            raise ValueError(f"a tensor is {t.dtype} on {t.device}, expected {dt} on {like.device}")
-    return dev
-
-
-def _code(dt: torch.dtype) -> int:
-    return _CODE[dt] if dt in _CODE else dtype_code(dt)
-
-
-def _rows(t: torch.Tensor, n: int) -> torch.Tensor:
-    """t [..., n] as [rows, n] with contiguous values (a view where its strides allow one)."""
-    if t.dim() != 2:
-        t = t.reshape(t.numel() // n if n else math.prod(t.shape[:-1]), n)
-    return t if n <= 1 or t.stride(1) == 1 else t.contiguous()
-
-
-def _separate(t: torch.Tensor) -> bool:
-    """Whether no two elements of t share memory (by its strides)."""
-    extent = 1
-    for st, n in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n > 1):
-        if st < extent:
-            return False
-        extent = st * n
-    return True
-
-
-def _rotary_side(x: torch.Tensor, out: torch.Tensor) -> RotarySide:
-    xb, xl, xh, _ = x.stride()
-    ob, ol, oh, _ = out.stride()
-    return RotarySide(x.data_ptr(), out.data_ptr(), x.shape[2], xb, xl, xh, ob, ol, oh)
-
-
-def _rotary_call(dev: int, q: torch.Tensor, k, q_out: torch.Tensor, k_out, positions: torch.Tensor, angles, rd: int,
-                 factor: float, interleaved: bool, inverse: bool):
-    """gsa_rotary on tensors that fit one another (as rotary checks them, and autograd its gradients)."""
-    B, L, _, D = q.shape
-    if q.stride(3) != 1:
-        q = q.contiguous()
-    side_k = None
-    if k is not None:
-        if k.stride(3) != 1:
-            k = k.contiguous()
-        side_k = C.byref(_rotary_side(k, k_out))
-    _run(dev, "gsa_rotary", _CODE[q.dtype], B, L, D, rd, C.byref(_rotary_side(q, q_out)), side_k, positions.data_ptr(),
-         positions.stride(0) if positions.shape[0] > 1 else 0, positions.stride(1), *angles, factor, interleaved,
-         inverse)
-
-
 def rotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq=None, factor: float = 1.0, interleaved: bool = False,
-           inverse: bool = False, out=None, tables=None, rotary_dim=None):
+           inverse: bool = False, out=None, tables=None, rotary_dim: int = 0):
     """q [B, L, H, D] and k [B, L, Hk, D] (or None) with the first ``2 * len(inv_freq)`` values of every
-    head rotated to ``positions`` ([B, L], [1, L] or [L]; int64): (q', k').
+    head rotated to ``positions`` ([B, L], [1, L] or [L] integers): (q', k').
 
     The angles are ``positions * inv_freq`` in 64 bits; ``tables=(cos, sin)`` [rows, >= rotary_dim/2] with
     ``rotary_dim`` takes their sines and cosines from tables instead.  Both are multiplied by ``factor``.
     Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``; ``inverse`` applies the transpose (the
     backward pass).  ``out=(q_out, k_out)`` receives the results, for example K in a cache's slots; an output may
     be its input itself (rotated in place) but may not overlap an input otherwise."""
-    dev = _check(q, k)
-    _code(q.dtype)
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
-        raise ValueError(f"rotary takes q [B, L, H, D] and k [B, L, Hk, D], got {tuple(q.shape)} and "
-                         f"{None if k is None else tuple(k.shape)}")
-    B, L, H, D = q.shape
-    angles = (None, None, None, 0, 0, 0)
-    if tables is not None:
-        cos, sin = tables
-        if (cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride() or cos.stride(1) != 1
-                or cos.dtype != sin.dtype or rotary_dim is None or cos.shape[1] < rotary_dim // 2
-                or cos.get_device() != dev or sin.get_device() != dev):
-            raise ValueError("rotary tables are two [rows, >= rotary_dim/2] tensors of the same strides beside q")
-        rd = rotary_dim
-        angles = (None, cos.data_ptr(), sin.data_ptr(), dtype_code(cos.dtype), cos.stride(0), cos.shape[0])
-    else:
-        if inv_freq is None or inv_freq.dim() != 1 or inv_freq.get_device() != dev:
-            raise ValueError("rotary takes inv_freq [rotary_dim/2] beside q")
-        rd = 2 * inv_freq.shape[0]
-        if inv_freq.dtype is not torch.float64 or not inv_freq.is_contiguous():
-            inv_freq = inv_freq.double().contiguous()
-        angles = (inv_freq.data_ptr(), None, None, 0, 0, 0)
-    if rd < 2 or rd > D or rd % 2 or D > 1024 or H + (0 if k is None else k.shape[2]) > 1024:
-        raise ValueError(f"rotary: rotary_dim {rd} of head dim {D}, at most 1024 wide and 1024 heads")
-    if positions.dim() == 1:
-        positions = positions.unsqueeze(0)
-    if positions.dim() != 2 or positions.shape[1] != L or positions.shape[0] not in (1, B):
-        raise ValueError(f"positions {tuple(positions.shape)} for {B} sequences of {L} tokens")
-    if positions.dtype is not torch.int64:
-        if positions.dtype.is_floating_point or positions.dtype == torch.bool:
-            raise ValueError("positions are integers")
-        positions = positions.long()
-    if positions.get_device() != dev:
-        raise ValueError(f"positions on {positions.device}, expected {q.device}")
-    if out is None:
-        q_out, k_out = _like(q), None if k is None else _like(k)
-    else:
-        q_out, k_out = out
-        for x, o in ((q, q_out), (k, k_out)):
-            if (x is None) != (o is None) or (x is not None and (
-                    o.shape != x.shape or o.dtype is not x.dtype or o.get_device() != dev
-                    or (o.shape[3] > 1 and o.stride(3) != 1) or not (o.is_contiguous() or _separate(o)))):
-                raise ValueError("rotary: out tensors have their inputs' shape, dtype and device, contiguous values and "
-                                 "no two elements in one place")
-    if q.numel() == 0 and (k is None or k.numel() == 0):
-        return q_out, k_out
-    if H == 0 or (k is not None and k.shape[2] == 0):
-        raise ValueError("rotary: a tensor without heads")
-    _rotary_call(dev, q, k, q_out, k_out, positions, angles, rd, factor, interleaved, inverse)
-    return q_out, k_out
+    r = _lib.native().rotary(q, k, positions, inv_freq, factor, interleaved, inverse, out, tables, rotary_dim)
+    _after("rotary")
+    return r
 
 
 class PackedActivation:
@@ -796,93 +666,46 @@ class PackedActivation:
         """The values as a tensor of ``dtype`` (default: the packed tensor's)."""
         return unpack_e4m3(self, dtype)
 
-    def _args(self):
-        """(codes, row stride, scales, row stride) for the C ABI."""
-        n = self.shape[-1]
-        ld = (n + 15) // 16 * 16
-        p = self.data.data_ptr()
-        return p, ld, p + math.prod(self.shape[:-1]) * ld, (n + 31) // 32
-
 
 def pack_e4m3(x: torch.Tensor) -> PackedActivation:
     """x [..., n] in 8 bits."""
-    dev = _check(x)
-    if x.dim() == 0:
-        raise ValueError("pack_e4m3 takes a tensor with a last dimension")
-    code = _code(x.dtype)
-    n = x.shape[-1]
-    p = PackedActivation.empty(x.shape, x.dtype, x.device)
-    if x.numel():
-        x2 = _rows(x, n)
-        _run(dev, "gsa_pack_e4m3", code, x2.shape[0], n, x2.data_ptr(), x2.stride(0), *p._args())
+    p = PackedActivation(_lib.native().pack(x), x.shape, x.dtype)
+    _after("pack_e4m3")
     return p
 
 
 def unpack_e4m3(p: PackedActivation, dtype=None) -> torch.Tensor:
     """The values of a packed tensor, in its dtype or the given one."""
-    x = p.data.new_empty(p.shape, dtype=dtype or p.dtype)
-    code = _code(x.dtype)
-    if x.numel():
-        n = p.shape[-1]
-        _run(_check(x), "gsa_unpack_e4m3", code, x.numel() // n, n, *p._args(), x.data_ptr(), n)
+    x = _lib.native().unpack(p.data, p.shape, dtype or p.dtype)
+    _after("unpack_e4m3")
     return x
 
 
 def silu_mul_packed(gu: torch.Tensor):
     """(z, packed): z = silu(g) * u of gu [..., 2n] = (g, u), and (g, u) packed as [..., 2, n]."""
-    dev = _check(gu)
-    if gu.dim() == 0 or gu.shape[-1] % 2:
-        raise ValueError(f"silu_mul_packed takes [..., 2n], got {tuple(gu.shape)}")
-    code = _code(gu.dtype)
-    n = gu.shape[-1] // 2
-    lead = gu.shape[:-1]
-    z = gu.new_empty((*lead, n))
-    p = PackedActivation.empty((*lead, 2, n), gu.dtype, gu.device)
-    if z.numel():
-        g2 = _rows(gu, 2 * n)
-        _run(dev, "gsa_silu_mul_pack", code, g2.shape[0], n, g2.data_ptr(), g2.stride(0), z.data_ptr(), n, *p._args())
-    return z, p
+    z, data = _lib.native().silu_mul_packed(gu)
+    _after("silu_mul_packed")
+    s = z.shape
+    return z, PackedActivation(data, (*s[:-1], 2, s[-1]), z.dtype)
 
 
 def silu_mul_packed_backward(dz: torch.Tensor, packed: PackedActivation, want_z: bool = False):
     """(dgu [..., 2n], z or None) of silu_mul_packed from dz [..., n] and the packed (g, u); z is that of the packed
     values, for the weight gradient of the product that reads it."""
-    dev = _check(dz)
-    if len(packed.shape) < 2 or packed.shape[-2] != 2 or dz.shape != packed.shape[:-2] + packed.shape[-1:]:
-        raise ValueError(f"dz {tuple(dz.shape)} for packed {tuple(packed.shape)}")
-    if dz.dtype is not packed.dtype or packed.data.get_device() != dev:
-        raise ValueError(f"dz is {dz.dtype} on {dz.device}, packed {packed.dtype} on {packed.data.device}")
-    n = packed.shape[-1]
-    dgu = dz.new_empty((*dz.shape[:-1], 2 * n))
-    z = _like(dz) if want_z else None
-    if dz.numel():
-        d2 = _rows(dz, n)
-        _run(dev, "gsa_silu_mul_packed_backward", _code(dz.dtype), d2.shape[0], n, d2.data_ptr(), d2.stride(0),
-             *packed._args(), dgu.data_ptr(), 2 * n, _ptr(z), n)
-    return dgu, z
+    s = packed.shape
+    if len(s) < 2 or s[-2] != 2 or dz.shape != s[:-2] + s[-1:] or dz.dtype is not packed.dtype:
+        raise ValueError(f"dz {tuple(dz.shape)} {dz.dtype} for packed {s} {packed.dtype}")
+    r = _lib.native().silu_mul_packed_backward(dz, packed.data, want_z)
+    _after("silu_mul_packed_backward")
+    return r
 
 
 def add_rmsnorm_packed(x: torch.Tensor, a, weight: torch.Tensor, eps: float):
     """(h, y, packed, rstd): h = x + a (None when a is None: h is x), y = RMSNorm(h) * weight over the last
     dimension, h packed, and rstd [...] fp32 -- what rmsnorm_packed_backward needs."""
-    dev = _check(x, a, weight)
-    if x.dim() == 0 or x.shape[-1] == 0 or weight.shape != x.shape[-1:] or (a is not None and a.shape != x.shape):
-        raise ValueError(f"add_rmsnorm_packed: x {tuple(x.shape)}, a {None if a is None else tuple(a.shape)}, weight "
-                         f"{tuple(weight.shape)}")
-    code = _code(x.dtype)
-    d = x.shape[-1]
-    h = _like(x) if a is not None else None
-    y = _like(x)
-    rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    p = PackedActivation.empty(x.shape, x.dtype, x.device)
-    if x.numel():
-        x2 = _rows(x, d)
-        a2 = None if a is None else _rows(a, d)
-        w = weight.contiguous()
-        _run(dev, "gsa_add_rmsnorm_pack", code, x2.shape[0], d, x2.data_ptr(), x2.stride(0), _ptr(a2),
-             0 if a2 is None else a2.stride(0), w.data_ptr(), eps, _ptr(h), d, y.data_ptr(), d,
-             *p._args(), rstd.data_ptr())
-    return h, y, p, rstd
+    h, y, data, rstd = _lib.native().add_rmsnorm_packed(x, a, weight, eps)
+    _after("add_rmsnorm_packed")
+    return h, y, PackedActivation(data, y.shape, y.dtype), rstd
 
 
 def rmsnorm_packed_backward(dy: torch.Tensor, packed: PackedActivation, rstd: torch.Tensor, weight: torch.Tensor,
@@ -890,66 +713,24 @@ def rmsnorm_packed_backward(dy: torch.Tensor, packed: PackedActivation, rstd: to
     """(dx, dw or None, y or None) of y = RMSNorm(h) * weight from dy, the packed h and rstd; ``dh`` (the gradient
     that reaches h past the norm) is added to dx.  y is that of the packed h, for the weight gradients of the
     products that read it."""
-    dev = _check(dy, weight, dh)
-    if dy.shape != packed.shape or weight.shape != dy.shape[-1:] or (dh is not None and dh.shape != dy.shape) \
-            or rstd.shape != dy.shape[:-1] or rstd.dtype is not torch.float32 or dy.shape[-1] == 0:
-        raise ValueError(f"rmsnorm_packed_backward: dy {tuple(dy.shape)}, packed {tuple(packed.shape)}, weight "
-                         f"{tuple(weight.shape)}, rstd {tuple(rstd.shape)}")
-    if packed.dtype is not dy.dtype or packed.data.get_device() != dev or rstd.get_device() != dev:
-        raise ValueError(f"dy is {dy.dtype} on {dy.device}, packed {packed.dtype} on {packed.data.device}")
-    d = dy.shape[-1]
-    rows = dy.numel() // d
-    dx = _like(dy)
-    y = _like(dy) if want_y else None
-    if rows == 0:
-        return dx, (dy.new_zeros(d) if want_dw else None), y
-    dw = ws = None
-    nbytes = 0
-    if want_dw:
-        dw = dy.new_empty(d)
-        nbytes = _lib.lib().gsa_rmsnorm_packed_workspace_size(rows, d)
-        ws = rstd.new_empty(nbytes // 4)
-    d2 = _rows(dy, d)
-    h2 = None if dh is None else _rows(dh, d)
-    w, rstd = weight.contiguous(), rstd.contiguous()
-    _run(dev, "gsa_rmsnorm_packed_backward", _code(dy.dtype), rows, d, d2.data_ptr(), d2.stride(0), _ptr(h2),
-         0 if h2 is None else h2.stride(0), w.data_ptr(), *packed._args(), rstd.data_ptr(), dx.data_ptr(), d, _ptr(y), d, _ptr(dw), _ptr(ws), nbytes)
-    return dx, dw, y
+    if dy.shape != packed.shape or dy.dtype is not packed.dtype:
+        raise ValueError(f"dy {tuple(dy.shape)} {dy.dtype} for packed {packed.shape} {packed.dtype}")
+    r = _lib.native().rmsnorm_packed_backward(dy, packed.data, rstd, weight, dh, want_y, want_dw)
+    _after("rmsnorm_packed_backward")
+    return r
 
 
 def next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100, want_grad: bool = True):
     """(loss, grad or None): mean cross entropy of labels[:, t + 1] under logits[:, t] ([B, L, V]), fp32, and its
     gradient in the logits' dtype.  Labels equal to ignore_index do not count; without any that count the loss is NaN
     and the gradient 0."""
-    dev = _check(logits)
-    if logits.dim() != 3 or logits.shape[2] == 0 or labels.shape != logits.shape[:2]:
-        raise ValueError(f"next_token_loss takes logits [B, L, V] and labels [B, L], got {tuple(logits.shape)} and "
-                         f"{tuple(labels.shape)}")
-    if labels.get_device() != dev:
-        _cuda(labels)
-        raise ValueError(f"labels on {labels.device}, logits on {logits.device}")
-    if labels.dtype is not torch.int64:
-        if labels.dtype.is_floating_point or labels.dtype == torch.bool:
-            raise ValueError("labels are integers")
-        labels = labels.long()
-    code = _code(logits.dtype)
-    B, L, V = logits.shape
-    x = logits if V == 1 or logits.stride(2) == 1 else logits.contiguous()
-    loss = logits.new_empty((), dtype=torch.float32)
-    nbytes = _lib.lib().gsa_next_token_loss_workspace_size()
-    ws = logits.new_empty(nbytes, dtype=torch.uint8)
-    grad = _like(logits) if want_grad else None
-    _run(dev, "gsa_next_token_loss", code, B, L, V, x.data_ptr(), x.stride(0), x.stride(1), labels.data_ptr(),
-         labels.stride(0), labels.stride(1), int(ignore_index), loss.data_ptr(), _ptr(grad), L * V, V,
-         ws.data_ptr(), nbytes)
-    return loss, grad
+    r = _lib.native().next_token_loss(logits, labels, ignore_index, want_grad)
+    _after("next_token_loss")
+    return r
 
 
 def scale_(x: torch.Tensor, factor: torch.Tensor) -> torch.Tensor:
     """x *= factor in place, for a contiguous x and a one-element fp32 tensor factor; a factor of 1 leaves x unread."""
-    dev = _check(x)
-    if not x.is_contiguous() or factor.numel() != 1 or factor.dtype is not torch.float32 or factor.get_device() != dev:
-        raise ValueError("scale_ takes a contiguous tensor and a one-element fp32 factor on its device")
-    if x.numel():
-        _run(dev, "gsa_scale", _code(x.dtype), x.numel(), x.data_ptr(), factor.data_ptr())
+    _lib.native().scale_(x, factor)
+    _after("scale_")
     return x

@@ -12,7 +12,7 @@ the backward pass, and the next-token loss with its gradient in one pass.
                                        node that keeps 1 + 2 d_ffn / d_model packed values per value of the stream
   fused_next_token_loss                GSALlamaForCausalLM's loss (gsa_llama.py:323-336)
 
-Each runs on its tensors' device and current stream and can be captured into a CUDA graph (a backward pass that is
+The autograd functions are in csrc/torch_ops.cpp.  Each runs on its tensors' device and current stream and can be captured into a CUDA graph (a backward pass that is
 captured must not share its leaves with a graph of eager operations that is still alive: torch binds the leaves'
 accumulation to the stream of the first).  Second derivatives are not implemented.
 """
@@ -25,7 +25,7 @@ from typing import Any, Dict, Optional, Tuple
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import ops
+from . import _lib, ops
 from .ops import PackedActivation
 
 
@@ -92,35 +92,6 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[Dict[s
     return f.to(device) if device is not None else f, float(cfg.get("attention_factor", 1.0))
 
 
-class _Rotary(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, positions, inv_freq, factor, interleaved):
-        out = ops.rotary(q, k, positions, inv_freq, factor, interleaved)  # refuses what does not fit
-        if positions.dim() == 1:
-            positions = positions.unsqueeze(0)
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(positions.long(), inv_freq.double().contiguous())
-        ctx.how = (factor, interleaved)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dq, dk):
-        positions, inv_freq = ctx.saved_tensors
-        factor, interleaved = ctx.how
-        need = ctx.needs_input_grad
-        grads = [dq if need[0] else None, dk if need[1] else None]
-        given = [g for g in grads if g is not None]
-        if given and given[0].numel():
-            q, k = given[0], given[1] if len(given) > 1 else None
-            q_out, k_out = ops._like(q), None if k is None else ops._like(k)
-            ops._rotary_call(q.get_device(), q, k, q_out, k_out, positions, (inv_freq.data_ptr(), None, None, 0, 0, 0),
-                             2 * inv_freq.shape[0], factor, interleaved, True)
-            outs = iter((q_out, k_out))
-            grads = [None if g is None else next(outs) for g in grads]
-        return grads[0], grads[1], None, None, None, None
-
-
 def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Tensor, inv_freq: torch.Tensor,
                  attention_factor: float = 1.0, interleaved: bool = False, out=None):
     """(q', k'): q [B, L, H, D] and k [B, L, Hk, D] (or None) rotated to ``positions`` ([B, L], [1, L] or [L] integers)
@@ -132,7 +103,7 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise NotImplementedError("apply_rotary writes into given tensors without autograd only")
-        return _Rotary.apply(q, k, positions, inv_freq, attention_factor, interleaved)
+        return _lib.native().rotary_autograd(q, k, positions, inv_freq, attention_factor, interleaved)
     return ops.rotary(q, k, positions, inv_freq, attention_factor, interleaved, out=out)
 
 
@@ -144,53 +115,18 @@ def pack_activation(x: torch.Tensor) -> PackedActivation:
     return ops.pack_e4m3(x)
 
 
-class _PackedSiluMul(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, gu):
-        z, p = ops.silu_mul_packed(gu)
-        ctx.save_for_backward(p.data)
-        ctx.form = (p.shape, p.dtype)
-        return z
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dz):
-        return ops.silu_mul_packed_backward(dz, PackedActivation(ctx.saved_tensors[0], *ctx.form))[0]
-
-
 def packed_silu_mul(gu: torch.Tensor) -> torch.Tensor:
     """silu(g) * u of gu [..., 2n] = (g, u); the backward pass reads (g, u) from 8 bits."""
     if torch.is_grad_enabled() and gu.requires_grad:
-        return _PackedSiluMul.apply(gu)
+        return _lib.native().silu_mul_autograd(gu)
     return ops.silu_mul_packed(gu)[0]
-
-
-class _PackedAddRMSNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, a, weight, eps):
-        ctx.set_materialize_grads(False)
-        h, y, p, rstd = ops.add_rmsnorm_packed(x, a, weight, eps)
-        ctx.save_for_backward(p.data, rstd, weight)
-        ctx.form = (p.shape, p.dtype)
-        return h, y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dh, dy):
-        data, rstd, weight = ctx.saved_tensors
-        if dy is None:
-            dx, dw = dh, None
-        else:
-            dx, dw, _ = ops.rmsnorm_packed_backward(dy, PackedActivation(data, *ctx.form), rstd, weight, dh=dh,
-                                                    want_dw=ctx.needs_input_grad[2])
-        return (dx if ctx.needs_input_grad[0] else None, dx if ctx.needs_input_grad[1] else None, dw, None)
 
 
 def packed_add_rmsnorm(x: torch.Tensor, a: Optional[torch.Tensor], weight: torch.Tensor, eps: float):
     """(h, y): h = x + a (x itself when a is None) and y = RMSNorm(h) * weight over the last dimension; the
     backward pass reads h from 8 bits."""
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, a, weight)):
-        h, y = _PackedAddRMSNorm.apply(x, a, weight, eps)
+        h, y = _lib.native().add_rmsnorm_autograd(x, a, weight, eps)
     else:
         h, y, _, _ = ops.add_rmsnorm_packed(x, a, weight, eps)
     return (x if a is None else h), y
@@ -245,28 +181,10 @@ def packed_mlp_block(x: torch.Tensor, a: Optional[torch.Tensor], weight: torch.T
 # ---------------------------------------------------------------------------------------------
 # The loss
 # ---------------------------------------------------------------------------------------------
-class _NextTokenLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, labels, ignore_index):
-        loss, ctx.grad = ops.next_token_loss(logits, labels, ignore_index)
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, d_loss):
-        grad, ctx.grad = ctx.grad, None
-        if grad is None:
-            raise RuntimeError("fused_next_token_loss: its gradient was handed out by an earlier backward pass; call it "
-                               "again for another")
-        ops._run(grad.get_device(), "gsa_scale", ops._CODE[grad.dtype], grad.numel(), grad.data_ptr(),
-                 d_loss.data_ptr())
-        return grad, None, None
-
-
 def fused_next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """Mean cross entropy (fp32) of the token at t + 1 under logits[:, t]; labels of ``ignore_index`` do not count
     (NaN where none counts).  Under autograd the gradient is formed together with the loss, in one reading of the
     logits, and handed out by the first backward pass (a second one through the same loss is refused)."""
     if torch.is_grad_enabled() and logits.requires_grad:
-        return _NextTokenLoss.apply(logits, labels, ignore_index)
+        return _lib.native().loss_autograd(logits, labels, ignore_index)
     return ops.next_token_loss(logits, labels, ignore_index, want_grad=False)[0]
