@@ -19,19 +19,26 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// sigma(x) = 1 / (1 + e^-x), off by a few units over the whole range, the subnormal tail included (z = g sigma(g) keeps
-// its relative accuracy there).
-__device__ __forceinline__ float sigmoid32(float x) {
-  float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + expf(-x)));
+// 4 sigma(x) = 1 / ((1 + e^-x) / 4): the quarter keeps the reciprocal in the normal range for all e^-x that are, so that
+// x sigma(x) has its relative accuracy over the whole range (a plain fast reciprocal gives 0 under 2^-126).  e^-x is
+// 2^t times 2^lo with t = -x log2 e rounded and lo what that lost; beyond +-1e4 it is 0 or infinite in any case.
+__device__ __forceinline__ float sigmoid_times4(float x) {
+  constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.925963e-8f, kLn2 = 0.693147181f;  // log2 e as a sum of two
+  const float c = fminf(fmaxf(x, -1e4f), 1e4f);
+  const float t = -c * kLog2e, lo = fmaf(-c, kLog2eLow, fmaf(-c, kLog2e, -t));
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  e *= fmaf(lo, kLn2, 1.0f);
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.25f, 0.25f)));
   return r;
 }
+__device__ __forceinline__ float silu_mul(float g, float u) { return 0.25f * g * sigmoid_times4(g) * u; }
 
 struct SwigluGrad {
   float dg, du, z;
 };
 __device__ __forceinline__ SwigluGrad swiglu_grad(float dz, float g, float u) {
-  const float sig = sigmoid32(g), silu = g * sig;
+  const float s4 = sigmoid_times4(g), sig = 0.25f * s4, silu = 0.25f * g * s4;
   return {dz * u * (sig * (1.0f + g * (1.0f - sig))), dz * silu, silu * u};
 }
 
@@ -82,7 +89,7 @@ __global__ void __launch_bounds__(kThreads) unpack16_kernel(const Cut c, const u
 
 // gu rows hold g then u; the packed rows 2r and 2r + 1 are row r's g and u.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) silu_mul_pack16_kernel(const Cut c, const T* gu, int64_t gu_ld, T* z,
+__global__ void __launch_bounds__(kThreads, 4) silu_mul_pack16_kernel(const Cut c, const T* gu, int64_t gu_ld, T* z,
                                                                    int64_t z_ld, uint8_t* codes, int64_t c_ld,
                                                                    uint8_t* scales, int64_t s_ld) {
   const Place p = place_of(c);
@@ -99,7 +106,7 @@ __global__ void __launch_bounds__(kThreads) silu_mul_pack16_kernel(const Cut c, 
   if (p.live) {
     float o[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) o[k] = g[k] * sigmoid32(g[k]) * u[k];
+    for (int k = 0; k < 16; ++k) o[k] = silu_mul(g[k], u[k]);
     store_half(z + p.r * z_ld + p.i, o);
   }
   uint4 qg, qu;
@@ -202,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) silu_mul_pack_kernel(const Cut c, co
     int sg, su;
     const uint32_t cg = pack_lane(g[k], &sg), cu = pack_lane(u[k], &su);  // by all lanes
     if (i + k * kGroup < c.n) {
-      z[r * z_ld + i + k * kGroup] = from_float<T>(g[k] * sigmoid32(g[k]) * u[k]);
+      z[r * z_ld + i + k * kGroup] = from_float<T>(silu_mul(g[k], u[k]));
       cp[k * kGroup] = (uint8_t)cg;
       cp[c_ld + k * kGroup] = (uint8_t)cu;
       if ((threadIdx.x & 31) == 0) {
