@@ -80,6 +80,11 @@ void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
 Tensor fresh(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
+// A tensor that the caller handed in has been written: graphs that saved it notice.
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 int64_t rows_of(at::IntArrayRef shape) {  // all but the last dimension
   int64_t n = 1;
   for (size_t i = 0; i + 1 < shape.size(); ++i) n *= shape[i];
@@ -127,6 +132,7 @@ Tensor pack(const Tensor& x) {
 
 Tensor unpack(const Tensor& data, const std::vector<int64_t>& shape, at::ScalarType dtype) {
   on_gpu(data);
+  TORCH_CHECK_VALUE(!shape.empty(), "a packed tensor has a last dimension");
   const int code = code_of(dtype);
   const On on(data);
   Tensor x = at::empty(shape, data.options().dtype(dtype));
@@ -355,6 +361,10 @@ Pair rotary(const Tensor& q, const optional<Tensor>& k, const Tensor& positions,
   }
   if (q.numel() == 0 && (!k || k->numel() == 0)) return {q_out, k_out};
   rotary_call(q, k, q_out, k_out, pos, a);
+  if (out) {
+    written(q_out);
+    if (k_out) written(*k_out);
+  }
   return {q_out, k_out};
 }
 
@@ -497,6 +507,7 @@ void scale_(const Tensor& x, const Tensor& factor) {
                     "scale_ takes a contiguous tensor and a one-element fp32 factor");
   const On on(x);
   ok("gsa_scale", api.scale(code_of(x.scalar_type()), x.numel(), ptr(x), factor.data_ptr<float>(), on.stream));
+  written(x);
 }
 
 struct LossFn : torch::autograd::Function<LossFn> {

@@ -675,6 +675,132 @@ def test_captured_training_step(cuda_ok):
     assert all(torch.equal(a, b) for a, b in zip(out, want))
 
 
+def test_refusals(cuda_ok):
+    """What does not fit together is refused before any launch: shapes, dtypes, devices, overlapping outputs, second
+    derivatives, an output under autograd."""
+    import gsa_b200 as gsa
+    from gsa_b200 import _lib, ops
+
+    q, k = _randn(1, 2, 6, 4, 16), _randn(2, 2, 6, 2, 16)
+    pos = torch.arange(6, device=DEV)
+    freq, _ = gsa.rotary_frequencies(16, device=DEV)
+    bad = [
+        (q[0], k, pos, freq), (q, k[:, :5], pos, freq), (q, k[..., :8], pos, freq), (q, k.bfloat16(), pos, freq),
+        (q, k, pos[:5], freq), (q, k, pos.expand(3, 6), freq), (q, k, pos.float(), freq), (q, k, pos > 2, freq),
+        (q, k, pos, freq.view(2, 4)), (q, k, pos, gsa.rotary_frequencies(18, device=DEV)[0]), (q, k, pos, freq[:0]),
+        (q[:, :, :0], k, pos, freq), (_randn(3, 1, 6, 1000, 16), _randn(3, 1, 6, 25, 16), pos, freq),
+        (_randn(3, 1, 6, 1, 1026), None, pos, freq),
+    ]
+    for args in bad:
+        with pytest.raises(ValueError):
+            gsa.apply_rotary(*args)
+    o = torch.empty_like(q)
+    for out in ((o, None), (o[:1].expand_as(q), torch.empty_like(k)), (o.bfloat16(), torch.empty_like(k)), (o[..., :8], torch.empty_like(k)),
+                (o.transpose(2, 3).contiguous().transpose(2, 3), torch.empty_like(k)),
+                (torch.empty(400, device=DEV).as_strided(q.shape, (96, 16, 8, 1)), torch.empty_like(k))):
+        with pytest.raises(ValueError):
+            gsa.apply_rotary(q, k, pos, freq, out=out)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        gsa.apply_rotary(q, k, pos.cpu(), freq)
+    with pytest.raises(NotImplementedError):
+        gsa.apply_rotary(q.half(), None, pos, freq)
+    leaf = q.clone().requires_grad_(True)
+    with pytest.raises(NotImplementedError):
+        gsa.apply_rotary(leaf, k, pos, freq, out=(o, torch.empty_like(k)))
+    with pytest.raises(ValueError):
+        ops.rotary(q, k, pos, tables=(torch.ones(8, 4, device=DEV), torch.ones(8, 4, device=DEV)), rotary_dim=16)
+    x, w = _randn(4, 5, 32), torch.ones(32, device=DEV)
+    for call in (lambda: gsa.pack_activation(x.half()), lambda: gsa.packed_silu_mul(x.half()),
+                 lambda: gsa.packed_add_rmsnorm(x.half(), None, w.half(), 1e-5),
+                 lambda: gsa.pack_activation(x).unpack(torch.float16),
+                 lambda: gsa.fused_next_token_loss(x.half()[None], torch.zeros(1, 5, device=DEV, dtype=torch.long))):
+        with pytest.raises(NotImplementedError):
+            call()
+    p = gsa.pack_activation(x)
+    z, pg = ops.silu_mul_packed(x)
+    h, y, ph, rstd = ops.add_rmsnorm_packed(x, x, w, 1e-5)
+    lg, lab = _randn(5, 2, 6, 10), torch.zeros(2, 6, device=DEV, dtype=torch.long)
+    for call in (lambda: gsa.pack_activation(x[0, 0]), lambda: gsa.PackedActivation(p.data[:-1], p.shape, p.dtype).unpack(),
+                 lambda: gsa.PackedActivation(p.data, (), p.dtype).unpack(), lambda: gsa.packed_silu_mul(x[:, :31]),
+                 lambda: ops.silu_mul_packed_backward(x, pg), lambda: ops.silu_mul_packed_backward(z.bfloat16(), pg),
+                 lambda: ops.silu_mul_packed_backward(z, p), lambda: gsa.packed_add_rmsnorm(x, x[:4], w, 1e-5),
+                 lambda: gsa.packed_add_rmsnorm(x, None, w[:31], 1e-5), lambda: gsa.packed_add_rmsnorm(x, None, w.bfloat16(), 1e-5),
+                 lambda: gsa.packed_add_rmsnorm(x[:, :0], None, w[:0], 1e-5), lambda: ops.rmsnorm_packed_backward(y[:4], ph, rstd, w),
+                 lambda: ops.rmsnorm_packed_backward(y, ph, rstd[:4], w), lambda: ops.rmsnorm_packed_backward(y, ph, rstd.double(), w),
+                 lambda: ops.rmsnorm_packed_backward(y, ph, rstd, w, dh=y[:4]), lambda: gsa.fused_next_token_loss(lg[0], lab),
+                 lambda: gsa.fused_next_token_loss(lg, lab[:, :5]), lambda: gsa.fused_next_token_loss(lg, lab.float()),
+                 lambda: gsa.fused_next_token_loss(lg[..., :0], lab), lambda: ops.scale_(lg[..., ::2], rstd[0]),
+                 lambda: ops.scale_(lg, rstd)):
+        with pytest.raises(ValueError):
+            call()
+    # a packed buffer off the alignment of its codes
+    odd = torch.empty(p.data.numel() + 1, device=DEV, dtype=torch.uint8)[1:]
+    with pytest.raises(_lib.GSAError):
+        gsa.PackedActivation(odd, p.shape, p.dtype).unpack()
+    # second derivatives
+    gu = _randn(6, 3, 64).requires_grad_(True)
+    with pytest.raises(NotImplementedError, match="second derivatives"):
+        torch.autograd.grad(gsa.packed_silu_mul(gu).sum(), gu, create_graph=True)
+    ops.check_device_error()
+
+
+def test_tensors_written_in_place_are_noticed(cuda_ok):
+    """A tensor that another graph saved and apply_rotary then overwrites: that graph's backward pass refuses."""
+    import gsa_b200 as gsa
+
+    q = _randn(1, 1, 4, 2, 16)
+    w = torch.ones_like(q).requires_grad_(True)
+    y = (w * q).sum()
+    freq, _ = gsa.rotary_frequencies(16, device=DEV)
+    with torch.no_grad():
+        gsa.apply_rotary(q, None, torch.arange(4, device=DEV), freq, out=(q, None))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+def test_offsets_past_32_bits(cuda_ok):
+    """The last rows of tensors of more than 2^31 elements, and tokens 2^31 elements apart."""
+    import gsa_b200 as gsa
+
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    bf = torch.bfloat16
+    rows, n = 140000, 16384
+    x = torch.zeros(rows, n, device=DEV, dtype=bf)
+    x[-3:] = _randn(1, 3, n, dtype=bf)
+    p = gsa.pack_activation(x)
+    assert torch.equal(p.unpack()[-3:], gsa.pack_activation(x[-3:].clone()).unpack())
+    z, pg = gsa.ops.silu_mul_packed(x)
+    z2, pg2 = gsa.ops.silu_mul_packed(x[-3:].clone())
+    assert torch.equal(z[-3:], z2)
+    dgu, _ = gsa.ops.silu_mul_packed_backward(z, pg)
+    assert torch.equal(dgu[-3:], gsa.ops.silu_mul_packed_backward(z2, pg2)[0])
+    del dgu, z, pg
+    w = torch.ones(n, device=DEV, dtype=bf)
+    _, y, ph, rstd = gsa.ops.add_rmsnorm_packed(x, None, w, 1e-5)
+    _, y2, ph2, rstd2 = gsa.ops.add_rmsnorm_packed(x[-3:].clone(), None, w, 1e-5)
+    assert torch.equal(y[-3:], y2) and torch.equal(rstd[-3:], rstd2)
+    dx = gsa.ops.rmsnorm_packed_backward(y, ph, rstd, w, want_dw=False)[0]
+    assert torch.equal(dx[-3:], gsa.ops.rmsnorm_packed_backward(y2, ph2, rstd2, w, want_dw=False)[0])
+    del dx, y, ph, p
+    logits = x.view(1, -1)[:, :128256 * 17000].view(1, 17000, 128256)
+    logits[0, -2] = _randn(2, 128256, dtype=bf)
+    labels = torch.full((1, 17000), -100, device=DEV)
+    labels[0, -1] = 77
+    loss, grad = gsa.ops.next_token_loss(logits, labels)
+    loss2, grad2 = gsa.ops.next_token_loss(logits[:, -2:].clone(), labels[:, -2:])
+    assert torch.equal(loss, loss2) and torch.equal(grad[:, -2:], grad2) and bool((grad[0, 5] == 0).all())
+    del logits, grad, x
+    far = torch.zeros((1 << 32) + 4096, device=DEV, dtype=bf)
+    q = far.as_strided((1, 3, 2, 64), (0, 1 << 31, 64, 1))
+    q.copy_(_randn(3, 1, 3, 2, 64, dtype=bf))
+    pos, (freq, _) = torch.arange(3, device=DEV) * 999, gsa.rotary_frequencies(64, device=DEV)
+    want = gsa.apply_rotary(q.clone(), None, pos, freq)[0]
+    assert torch.equal(gsa.apply_rotary(q, None, pos, freq)[0], want)
+    gsa.apply_rotary(q, None, pos, freq, out=(q, None))
+    assert torch.equal(q, want)
+
+
 # -- together -----------------------------------------------------------------------------------
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("rows,d,n", [(5, 48, 33), (64, 256, 512)])
@@ -769,6 +895,23 @@ def test_causal_lm_packed_training_step(cuda_ok, dtype):
     m.zero_grad(set_to_none=True)
     again = m(ids, labels=ids)
     assert torch.equal(again.loss, plain.loss)
+
+
+def test_packed_training_with_gradient_checkpointing(cuda_ok):
+    """Recomputing the layers in the backward pass gives the same gradients."""
+    m = _lm(torch.float32)
+    m.enable_packed_training()
+    ids = torch.randint(0, 384, (2, 32), generator=torch.Generator().manual_seed(2)).to(DEV)
+    grads = []
+    for again in (False, True):
+        m.model.gradient_checkpointing = again
+        m.zero_grad(set_to_none=True)
+        m(ids, labels=ids).loss.backward()
+        grads.append({n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None})
+    assert grads[0].keys() == grads[1].keys()
+    for name, g in grads[0].items():
+        # dK and dV of the sparse attention are added by atomics, in an order of their own each time
+        assert float((grads[1][name] - g).norm()) <= 1e-4 * float(g.norm()), name
 
 
 def test_packed_training_holds_less(cuda_ok):
