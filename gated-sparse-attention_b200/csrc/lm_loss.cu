@@ -327,28 +327,35 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (i0 + j * kRow < walk.pieces) raw[j] = xp[i0 + j * kRow];
+    // the largest of all of them first: one rescaling of the sum, and exponentials that wait for nothing
+    Piece<T> most;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j * kRow < walk.pieces) most.meet(raw[j]);
+    const float here = most.top();
+    if (here <= kLow) continue;
+    if (here > top) {
+      top = here;
+      const float up = here * kLog2e;
+      p.s *= exp2_fast(p.m - up);
+      p.m = up;
+    }
+    const uint64_t neg_m = pair_of(-p.m, -p.m);
+    uint64_t sum[n / 2];
+#pragma unroll
+    for (int k = 0; k < n / 2; ++k) sum[k] = 0;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) {
       if (i0 + j * kRow >= walk.pieces) break;
-      Piece<T> most;
-      most.meet(raw[j]);
-      const float here = most.top();
-      if (here <= kLow) continue;
-      if (here > top) {
-        top = here;
-        const float up = here * kLog2e;
-        p.s *= exp2_fast(p.m - up);
-        p.m = up;
-      }
       uint64_t v[n / 2];
       Piece<T>::get(raw[j], v);
-      const uint64_t neg_m = pair_of(-p.m, -p.m);
-      uint64_t sum = weight2(v[0], neg_m);
 #pragma unroll
-      for (int k = 1; k < n / 2; ++k) sum = add2(sum, weight2(v[k], neg_m));
-      const float2 both = split(sum);
-      p.s += both.x + both.y;
+      for (int k = 0; k < n / 2; ++k) sum[k] = add2(sum[k], weight2(v[k], neg_m));
     }
+#pragma unroll
+    for (int k = 1; k < n / 2; ++k) sum[0] = add2(sum[0], sum[k]);
+    const float2 both = split(sum[0]);
+    p.s += both.x + both.y;
   }
   for (int e = lane; e < walk.edges; e += kRow) {
     const float v = to_float(x[walk.edge(e)]);
@@ -368,7 +375,7 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
   const float loss = bad || m == INFINITY ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
   if (!g) return loss;
   const float inv = isnan(loss) ? loss : inv_count / s;
-  const int at = bad ? -1 : (int)target - walk.first;  // in 16-byte pieces' values
+  const int at = bad ? -1 : (int)target - walk.first;  // among the pieces' values
   const uint64_t neg_m = pair_of(-m, -m), inv2 = pair_of(inv, inv);
   for (int i0 = lane; i0 < walk.pieces; i0 += kAhead * kRow) {
     if (!once) {
@@ -389,15 +396,12 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
         q[2 * k] = both.x;
         q[2 * k + 1] = both.y;
       }
-      const int k0 = at - i * n;
-      if (k0 >= 0 && k0 < n) {
-#pragma unroll
-        for (int k = 0; k < n; ++k)
-          if (k == k0) q[k] -= inv_count;
-      }
       __stcs(gp + i, Piece<T>::set(q));
     }
   }
+  // the label's value again, one less, by the thread that stored it
+  if (at >= 0 && at < walk.pieces * n && at / n % kRow == lane)
+    g[target] = from_float<T>(exp2_fast(fmaf(x_target, kLog2e, -m)) * inv - inv_count);
   for (int e = lane; e < walk.edges; e += kRow) {
     const int i = walk.edge(e);
     float q = exp2_fast(fmaf(to_float(x[i]), kLog2e, -m)) * inv;

@@ -315,8 +315,10 @@ extern "C" int gsa_rotary(int dtype, int64_t B, int64_t L, int32_t D, int32_t rd
   a.tab_rows = tab_rows;
   a.factor = factor;
   a.inverse = inverse;
-  int st = device_error_word(&a.err);
-  if (st) return st;
+  if (!inv_freq) {  // only a position outside the tables is an error of the device's
+    const int st = device_error_word(&a.err);
+    if (st) return st;
+  }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return dtype == GSA_DTYPE_BF16 ? launch_typed<__nv_bfloat16>(a, interleaved, s)
                                  : launch_typed<float>(a, interleaved, s);
