@@ -10,6 +10,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kernels.cuh"
 
 namespace gsa {
@@ -140,17 +142,211 @@ struct Half<float> {
   }
 };
 
-template <typename T>
-__device__ __forceinline__ void load_half(const T* p, float* v) {
-  Half<T> h;
-  h.load(p);
-  h.get(v);
+// ---------------------------------------------------------------------------------------------
+// Rows that are not whole multiples of 16 values, or not aligned to 32 bytes ("ragged"): a thread still holds 16
+// neighbouring ones.  It reads the aligned 16-byte pieces that they lie in and writes aligned pieces, of which two
+// neighbouring lanes share one: the right one puts it together.  Which register holds which value goes by the
+// row's offset, one of a few cases with code of its own, so that taking a value costs no shift beside its
+// conversion.  Only pieces at a row's ends and at a warp's go word by word.
+// ---------------------------------------------------------------------------------------------
+
+// Calls f with one of eight offsets, 0 to 7, at compile time.
+template <typename F>
+__device__ __forceinline__ void by_offset(int offset, F f) {
+  switch (offset) {
+    case 0: f(std::integral_constant<int, 0>()); break;
+    case 1: f(std::integral_constant<int, 1>()); break;
+    case 2: f(std::integral_constant<int, 2>()); break;
+    case 3: f(std::integral_constant<int, 3>()); break;
+    case 4: f(std::integral_constant<int, 4>()); break;
+    case 5: f(std::integral_constant<int, 5>()); break;
+    case 6: f(std::integral_constant<int, 6>()); break;
+    default: f(std::integral_constant<int, 7>());
+  }
 }
+
+// The values of a row that a thread holds (0 to 16), and whether the lanes beside it hold their neighbours.
+struct Spot {
+  int live;
+  bool left, right;
+};
+template <bool kRagged>
+__device__ __forceinline__ Spot spot_of(int64_t i, int64_t n, bool row) {
+  row = row && i < n;
+  if (!kRagged) return {row ? 16 : 0, false, false};
+  const int lane = threadIdx.x & 31;
+  return {row ? (int)min((int64_t)16, n - i) : 0, row && i > 0 && lane > 0, row && i + 16 < n && lane < 31};
+}
+
+// The bytes of a tensor: pieces that reach out of it are read value by value.
+struct Extent {
+  const char *lo, *hi;
+};
 template <typename T>
-__device__ __forceinline__ void store_half(T* p, const float* v) {
+__device__ __forceinline__ Extent extent_of(const T* x, int64_t rows, int64_t ld, int64_t n) {
+  return {reinterpret_cast<const char*>(x), reinterpret_cast<const char*>(x + (rows - 1) * ld + n)};
+}
+
+// 16 values as they are read, and their conversion.  Whole rows are loaded where the spot is live, several tensors under one
+// condition; ragged ones see to that themselves (measured: the other way round each is 5-10% slower).
+template <typename T, bool kRagged>
+struct HalfIn {
   Half<T> h;
-  h.set(v);
-  h.store(p);
+  __device__ __forceinline__ void zero() { h.zero(); }
+  template <bool kShared = false>
+  __device__ __forceinline__ void load(const T* p, const Spot& at, const Extent&) {
+    if (kShared)
+      h.load_shared(p);
+    else
+      h.load(p);
+  }
+  __device__ __forceinline__ void get(float* v, const Spot&) const { h.get(v); }
+};
+template <typename T>
+struct HalfIn<T, true> {
+  static constexpr int kSize = (int)sizeof(T), kPieces = kSize + 1;
+  uint32_t w[4 * kPieces];
+  int offset;  // of the first value in w, in bytes
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < 4 * kPieces; ++i) w[i] = 0;
+    offset = 0;
+  }
+  __device__ __forceinline__ void piece(int j, const char* q) {
+    const uint4 t = __ldg(reinterpret_cast<const uint4*>(q) + j);
+    w[4 * j] = t.x;
+    w[4 * j + 1] = t.y;
+    w[4 * j + 2] = t.z;
+    w[4 * j + 3] = t.w;
+  }
+  template <bool kShared = false>
+  __device__ __forceinline__ void load(const T* p, const Spot& at, const Extent& in) {
+    zero();
+    if (!at.live) return;
+    offset = (int)(reinterpret_cast<uintptr_t>(p) & 15);
+    const char* q = reinterpret_cast<const char*>(p) - offset;
+    if (q >= in.lo && q + 16 * kPieces <= in.hi) {
+#pragma unroll
+      for (int j = 0; j < kPieces - 1; ++j) piece(j, q);
+      if (offset) piece(kPieces - 1, q);
+      return;
+    }
+#pragma unroll
+    for (int b = 0; b < 16 * kPieces; b += kSize) {
+      if (b < offset || b >= offset + at.live * kSize) continue;
+      if (kSize == 2)
+        w[b / 4] |= (uint32_t)*reinterpret_cast<const uint16_t*>(q + b) << (b % 4 * 8);
+      else
+        w[b / 4] = *reinterpret_cast<const uint32_t*>(q + b);
+    }
+  }
+  __device__ __forceinline__ void get(float* v, const Spot& at) const {
+    if (kSize == 2) {
+      by_offset(offset / 2, [&](auto o) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          const int b = 2 * (decltype(o)::value + k);
+          v[k] = __uint_as_float(b % 4 ? w[b / 4] & 0xffff0000u : w[b / 4] << 16);
+        }
+      });
+    } else {
+      uint32_t t[18];
+#pragma unroll
+      for (int i = 0; i < 18; ++i) t[i] = offset & 8 ? w[(i + 2) % (4 * kPieces)] : w[i % (4 * kPieces)];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(offset & 4 ? t[i + 1] : t[i]);
+    }
+    if (at.live < 16)
+#pragma unroll
+      for (int k = 0; k < 16; ++k)
+        if (k >= at.live) v[k] = 0.f;
+  }
+};
+
+// 16 values as whole words from the start of the piece that they begin in, offset bytes before them; zeros around them.
+__device__ __forceinline__ void lay_out(const __nv_bfloat16*, const float* v, int offset, uint32_t* t) {
+  by_offset(offset / 2, [&](auto o) {
+#pragma unroll
+    for (int i = 0; i < 12; ++i) {
+      const int k = 2 * i - decltype(o)::value;  // the low value's
+      const __nv_bfloat162 h = __floats2bfloat162_rn(k >= 0 && k < 16 ? v[k & 15] : 0.f,
+                                                     k >= -1 && k < 15 ? v[(k + 1) & 15] : 0.f);
+      t[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+  });
+}
+__device__ __forceinline__ void lay_out(const float*, const float* v, int offset, uint32_t* t) {
+  by_offset(offset / 4, [&](auto o) {
+#pragma unroll
+    for (int i = 0; i < 24; ++i) {
+      const int k = i - decltype(o)::value;
+      t[i] = k >= 0 && k < 16 ? __float_as_uint(v[k & 15]) : 0u;
+    }
+  });
+}
+__device__ __forceinline__ void store_piece(char* p, const uint32_t (&w)[4]) {
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store_piece(char* p, const uint32_t (&w)[8]) {
+  store32(p, Words8{{w[0], w[1], w[2], w[3], w[4], w[5], w[6], w[7]}});
+}
+
+// Stores a thread's 16 values at p; ragged ones by every lane of the warp together, in pieces of eight values: fp32 ones
+// are whole sectors, which bf16's 16 bytes are not (but with sectors the registers' turns cost more: 85 us against 98 for
+// 32768 x 4090 unpacked; for fp32 it is 77 against 58).
+template <bool kRagged, typename T>
+__device__ __forceinline__ void put_values(T* p, const float* v, const Spot& at) {
+  if (!kRagged) {
+    if (!at.live) return;
+    Half<T> h;
+    h.set(v);
+    h.store(p);
+    return;
+  }
+  constexpr int kSize = (int)sizeof(T), kShift = kSize / 2, kBytes = 8 * kSize, kWords = kBytes / 4;
+  const int offset = (int)(reinterpret_cast<uintptr_t>(p) & (kBytes - 1));
+  uint32_t t[3 * kWords];
+  lay_out(p, v, offset, t);
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    const uint32_t before = __shfl_up_sync(0xffffffffu, t[2 * kWords + i], 1);
+    if (at.left) t[i] |= before;
+  }
+  char* q = reinterpret_cast<char*>(p) - offset;
+  const int b0 = at.left ? 0 : offset, b1 = at.right ? 2 * kBytes : offset + at.live * kSize;  // this lane's bytes
+  int parts = 0;  // pieces of which this lane has a part
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) w[i] = t[kWords * j + i];
+    if (b0 <= kBytes * j && b1 >= kBytes * (j + 1))
+      store_piece(q + kBytes * j, w);
+    else if (b0 < kBytes * (j + 1) && b1 > kBytes * j && b1 > b0)
+      parts |= 1 << j;
+  }
+  while (parts) {
+    const int j = __ffs(parts) - 1;
+    parts &= parts - 1;
+    uint32_t w[kWords];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      w[i] = t[i];
+#pragma unroll
+      for (int m = 1; m < 3; ++m) w[i] = j == m ? t[kWords * m + i] : w[i];
+    }
+    const int lo = max(b0 - kBytes * j, 0) >> kShift, hi = min(b1 - kBytes * j, kBytes) >> kShift;
+    const uint32_t mine = (1u << hi) - (1u << lo);
+    char* to = q + kBytes * j;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (!(mine >> k & 1u)) continue;
+      if (kSize == 2)
+        reinterpret_cast<uint16_t*>(to)[k] = (uint16_t)(w[k / 2] >> (k % 2 * 16));
+      else
+        reinterpret_cast<uint32_t*>(to)[k] = w[k % kWords];
+    }
+  }
 }
 
 // A group held by two neighbouring lanes (every lane of the warp calls this): the scale byte, and this lane's 16
@@ -196,6 +392,22 @@ __device__ __forceinline__ uint4 load_codes(const uint8_t* p) {
   asm("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
       : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
       : "l"(p));
+  return r;
+}
+// The same for a spot as HalfIn loads it; the codes behind a ragged row's end as zeros, whatever the buffer holds there.
+template <bool kRagged>
+__device__ __forceinline__ uint4 load_codes(const uint8_t* p, const Spot& at) {
+  if (kRagged && !at.live) return make_uint4(0, 0, 0, 0);
+  uint4 r = load_codes(p);
+  if (kRagged && at.live < 16) {
+    uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = min(max(at.live - 4 * i, 0), 4);
+      w[i] = k == 4 ? w[i] : w[i] & ((1u << (8 * k)) - 1u);
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
   return r;
 }
 __device__ __forceinline__ void store_codes(uint8_t* p, const uint4& c) {

@@ -7,11 +7,12 @@
 // before the norm, since the residual stream that the backward pass differentiates is what the tensor holds.
 //
 // Bound by the bytes that it moves: a row is held in registers, so every tensor is read once and written once.  A thread
-// holds 16 neighbouring values (half a group: 32-byte accesses, one shuffle for the scale) where rows are whole
-// multiples of that and aligned, else 16 values a row's threads apart (a group a warp).  A CTA takes a row, or a
+// holds 16 neighbouring values (half a group: 32-byte accesses, one shuffle for the scale), through 16-byte pieces where
+// rows are not whole multiples of that or not aligned (kRagged: packed.cuh).  A CTA takes a row, or a
 // warp one of up to 512 values (several, where rows are shorter still).  The backward pass keeps its CTAs for all rows:
 // each sums dw beside dx over its rows in order, and a last kernel adds the CTAs' sums in order.
 #include <algorithm>
+#include <type_traits>
 
 #include "packed.cuh"
 
@@ -21,8 +22,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kWarpRow = 512;   // values of a row that a warp holds
-constexpr int kLaneRow = 8192;  // values of an unaligned row that a CTA holds, 16 a thread
-constexpr int kMaxRow = 16384;  // values of an aligned row that a CTA holds, 16 or 32 a thread
+constexpr int kHalfRow = 8192;  // values of a row that a CTA holds at 16 a thread
+constexpr int kMaxRow = 16384;  // the same at 32
 
 struct NormFwd {
   int64_t rows, d;
@@ -79,34 +80,36 @@ __device__ __forceinline__ float rstd_of(float ss, const NormFwd& a) { return 1.
 // ---------------------------------------------------------------------------------------------
 // 16 neighbouring values a thread, kHalves times.
 // ---------------------------------------------------------------------------------------------
-template <typename T, bool kWarpRows, int kHalves, int kMaxThreads>
+template <typename T, bool kRagged, bool kWarpRows, int kHalves, int kMaxThreads>
 __global__ void __launch_bounds__(kMaxThreads) add_rmsnorm_pack16_kernel(const NormFwd a) {
   __shared__ float ws[32];
   const int lane = threadIdx.x & 31, per = kWarpRows ? 32 / a.lanes : 1;
   const int64_t r = kWarpRows ? ((int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5)) * per + lane / a.lanes : blockIdx.x;
   const int64_t i0 = (kWarpRows ? lane & (a.lanes - 1) : threadIdx.x) * 16;
   const int64_t step = (int64_t)blockDim.x * 16;  // between a thread's halves
+  const T *x = static_cast<const T*>(a.x), *add = static_cast<const T*>(a.a), *w = static_cast<const T*>(a.w);
   float v[kHalves][16], ss = 0.f;
 #pragma unroll
   for (int j = 0; j < kHalves; ++j) {
     const int64_t i = i0 + j * step;
-    const bool live = i < a.d && r < a.rows;
-    Half<T> hx, ha;
+    const Spot at = spot_of<kRagged>(i, a.d, r < a.rows);
+    HalfIn<T, kRagged> hx, ha;
     hx.zero();
     ha.zero();
-    if (live) {
-      hx.load(static_cast<const T*>(a.x) + r * a.x_ld + i);
-      if (a.a) ha.load(static_cast<const T*>(a.a) + r * a.a_ld + i);
+    if (kRagged || at.live) {
+      hx.load(x + r * a.x_ld + i, at, extent_of(x, a.rows, a.x_ld, a.d));
+      if (a.a) ha.load(add + r * a.a_ld + i, at, extent_of(add, a.rows, a.a_ld, a.d));
     }
-    hx.get(v[j]);
+    hx.get(v[j], at);
     if (a.a) {
       float t[16];
-      ha.get(t);
+      ha.get(t, at);
 #pragma unroll
       for (int k = 0; k < 16; ++k) v[j][k] += t[k];
-      hx.set(v[j]);
-      if (live && a.h) hx.store(static_cast<T*>(a.h) + r * a.h_ld + i);
-      hx.get(v[j]);
+      Half<T> sum;
+      sum.set(v[j]);
+      sum.get(v[j]);
+      if (a.h) put_values<kRagged>(static_cast<T*>(a.h) + r * a.h_ld + i, v[j], at);
     }
 #pragma unroll
     for (int k = 0; k < 16; ++k) ss = fmaf(v[j][k], v[j][k], ss);
@@ -116,28 +119,29 @@ __global__ void __launch_bounds__(kMaxThreads) add_rmsnorm_pack16_kernel(const N
 #pragma unroll
   for (int j = 0; j < kHalves; ++j) {
     const int64_t i = i0 + j * step;
-    const bool live = i < a.d && r < a.rows;
-    if (live) {
-      Half<T> hw;
-      hw.load_shared(static_cast<const T*>(a.w) + i);
+    const Spot at = spot_of<kRagged>(i, a.d, r < a.rows);
+    if (kRagged || at.live) {
+      HalfIn<T, kRagged> hw;
+      hw.zero();
+      if (kRagged || at.live) hw.template load<true>(w + i, at, extent_of(w, 1, 0, a.d));
       float t[16];
-      hw.get(t);
+      hw.get(t, at);
 #pragma unroll
       for (int k = 0; k < 16; ++k) t[k] = v[j][k] * rstd * t[k];
-      store_half(static_cast<T*>(a.y) + r * a.y_ld + i, t);
+      put_values<kRagged>(static_cast<T*>(a.y) + r * a.y_ld + i, t, at);
     }
     uint4 q;
     const int s = pack_half(v[j], &q);
-    if (!live) continue;
+    if (!at.live) continue;
     store_codes(a.codes + r * a.c_ld + i, q);
     if ((threadIdx.x & 1) == 0) a.scales[r * a.s_ld + i / kGroup] = (uint8_t)s;
   }
 }
 
 // What the backward pass reads of 16 values of a row.
-template <typename T>
+template <typename T, bool kRagged>
 struct RowIn {
-  Half<T> dy, dh;
+  HalfIn<T, kRagged> dy, dh;
   uint4 codes;
   float scale, rstd;
   __device__ __forceinline__ void load(const NormBwd& a, int64_t r, int64_t i) {
@@ -145,23 +149,24 @@ struct RowIn {
     dh.zero();
     codes = make_uint4(0, 0, 0, 0);
     scale = rstd = 0.f;
-    if (r >= a.rows || i >= a.d) return;
-    dy.load(static_cast<const T*>(a.dy) + r * a.dy_ld + i);
-    codes = load_codes(a.codes + r * a.c_ld + i);
-    if (a.dh) dh.load(static_cast<const T*>(a.dh) + r * a.dh_ld + i);
+    const Spot at = spot_of<kRagged>(i, a.d, r < a.rows);
+    if (!kRagged && !at.live) return;
+    const T *py = static_cast<const T*>(a.dy), *ph = static_cast<const T*>(a.dh);
+    dy.load(py + r * a.dy_ld + i, at, extent_of(py, a.rows, a.dy_ld, a.d));
+    codes = load_codes<kRagged>(a.codes + r * a.c_ld + i, at);
+    if (a.dh) dh.load(ph + r * a.dh_ld + i, at, extent_of(ph, a.rows, a.dh_ld, a.d));
+    if (!at.live) return;
     scale = pow2_of(a.scales[r * a.s_ld + i / kGroup]);
     rstd = a.rstd[r];
   }
 };
 
-// The columns' sums of a CTA whose warps held rows: acc[k] of column i + k, added over the warps in order.
-template <int K>
+// The columns' sums of a CTA whose warps held rows: acc[k] of column first + k, added over the warps in order.
 __device__ __forceinline__ void warp_rows_part(const NormBwd& a, const float* acc, float* part, float (*col)[kWarpRow],
-                                               int first, int stride, bool writes) {
+                                               int first, bool writes) {
   if (writes)
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (first + k * stride < kWarpRow) col[threadIdx.x >> 5][first + k * stride] = acc[k];
+    for (int k = 0; k < 16; ++k) col[threadIdx.x >> 5][first + k] = acc[k];
   __syncthreads();
   for (int c = threadIdx.x; c < a.d; c += kThreads) {
     float t = 0.f;
@@ -171,33 +176,52 @@ __device__ __forceinline__ void warp_rows_part(const NormBwd& a, const float* ac
   }
 }
 
+// A thread's 16 sums of a CTA's share of dw.
+template <bool kRagged>
+__device__ __forceinline__ void put_part(float* part, const float* acc, int live) {
+  if (kRagged) {
+#pragma unroll
+    for (int k = 0; k < 16; ++k)
+      if (k < live) part[k] = acc[k];
+  } else if (live) {
+#pragma unroll
+    for (int k = 0; k < 16; k += 4)
+      *reinterpret_cast<float4*>(part + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+  }
+}
+
 // Rows blockIdx.x, blockIdx.x + gridDim.x, ... (or as many for each warp); part[blockIdx.x] = the CTA's sum of dy x^ over
-// its rows, in that order.  The next row is loaded before this row's sum is waited for.
-template <typename T, bool kWarpRows>
+// its rows, in that order.  The next row is loaded before this row's sum is waited for; not so a
+// ragged one, for want of registers.
+template <typename T, bool kRagged, bool kWarpRows>
 __global__ void __launch_bounds__(kWarpRows ? kThreads : 512) rmsnorm_bwd16_kernel(const NormBwd a) {
   __shared__ float ws[2][32];
   __shared__ float col[kWarpRows ? kWarps : 1][kWarpRow];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per = kWarpRows ? 32 / a.lanes : 1;
   const int64_t i = (kWarpRows ? lane & (a.lanes - 1) : threadIdx.x) * 16;
-  Half<T> hw;
+  const Spot col_at = spot_of<kRagged>(i, a.d, true);
+  HalfIn<T, kRagged> hw;
   hw.zero();
-  if (i < a.d) hw.load_shared(static_cast<const T*>(a.w) + i);
+  if (kRagged || col_at.live)
+    hw.template load<true>(static_cast<const T*>(a.w) + i, col_at, extent_of(static_cast<const T*>(a.w), 1, 0, a.d));
   float acc[16];
 #pragma unroll
   for (int k = 0; k < 16; ++k) acc[k] = 0.f;
   const int64_t step = (int64_t)gridDim.x * (kWarpRows ? kWarps : 1) * per;
   int64_t base = (kWarpRows ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x) * per;
   const int slot = kWarpRows ? lane / a.lanes : 0;
-  RowIn<T> in;
-  in.load(a, base + slot, i);
+  RowIn<T, kRagged> in;
+  if (!kRagged) in.load(a, base + slot, i);
   const float inv_d = 1.0f / (float)a.d;
   for (int turn = 0; base < a.rows; ++turn, base += step) {
-    const RowIn<T> cur = in;
     const int64_t r = base + slot;
-    in.load(a, r + step, i);
+    if (kRagged) in.load(a, r, i);
+    const RowIn<T, kRagged> cur = in;
+    const Spot at = spot_of<kRagged>(i, a.d, r < a.rows);
+    if (!kRagged) in.load(a, r + step, i);
     float dy[16], xh[16], w[16];
-    cur.dy.get(dy);
-    hw.get(w);
+    cur.dy.get(dy, at);
+    hw.get(w, col_at);
     unpack_half(cur.codes, cur.scale, xh);
     float along = 0.f;
 #pragma unroll
@@ -207,16 +231,16 @@ __global__ void __launch_bounds__(kWarpRows ? kThreads : 512) rmsnorm_bwd16_kern
       acc[k] = fmaf(dy[k], xh[k], acc[k]);
     }
     along = row_sum<kWarpRows>(along, a.lanes, ws[turn & 1]) * inv_d;
-    if (i < a.d && r < a.rows) {
+    if (kRagged || at.live) {
       float dh[16];
-      cur.dh.get(dh);
+      cur.dh.get(dh, at);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         dh[k] += cur.rstd * (dy[k] * w[k] - xh[k] * along);
         xh[k] *= w[k];
       }
-      store_half(static_cast<T*>(a.dx) + r * a.dx_ld + i, dh);
-      if (a.y) store_half(static_cast<T*>(a.y) + r * a.y_ld + i, xh);
+      put_values<kRagged>(static_cast<T*>(a.dx) + r * a.dx_ld + i, dh, at);
+      if (a.y) put_values<kRagged>(static_cast<T*>(a.y) + r * a.y_ld + i, xh, at);
     }
   }
   if (!a.dw) return;
@@ -225,19 +249,22 @@ __global__ void __launch_bounds__(kWarpRows ? kThreads : 512) rmsnorm_bwd16_kern
     for (int o = a.lanes; o < 32; o <<= 1)  // the warp's rows side by side
 #pragma unroll
       for (int k = 0; k < 16; ++k) acc[k] += __shfl_xor_sync(0xffffffffu, acc[k], o);
-    warp_rows_part<16>(a, acc, part, col, (int)i, 1, lane < a.lanes);
-  } else if (i < a.d) {
-#pragma unroll
-    for (int k = 0; k < 16; k += 4)
-      *reinterpret_cast<float4*>(part + i + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+    warp_rows_part(a, acc, part, col, (int)i, lane < a.lanes);
+  } else {
+    put_part<kRagged>(part + i, acc, col_at.live);
   }
 }
 
 // Rows of more than 8192 values: 32 a thread.  Their sums of dw leave no registers to load ahead, or for the weights.
-template <typename T>
+template <typename T, bool kRagged>
 __global__ void __launch_bounds__(512) rmsnorm_bwd32_kernel(const NormBwd a) {
   __shared__ float ws[2][32];
   const int64_t step = (int64_t)blockDim.x * 16;
+  const T *py = static_cast<const T*>(a.dy), *ph = static_cast<const T*>(a.dh), *pw = static_cast<const T*>(a.w);
+  const Extent in_w = extent_of(pw, 1, 0, a.d);
+  Spot at[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) at[j] = spot_of<kRagged>(threadIdx.x * 16 + j * step, a.d, true);
   float acc[2][16];
 #pragma unroll
   for (int j = 0; j < 2; ++j)
@@ -247,7 +274,7 @@ __global__ void __launch_bounds__(512) rmsnorm_bwd32_kernel(const NormBwd a) {
   int turn = 0;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, ++turn) {
     const float rstd = a.rstd[r];
-    Half<T> hdy[2];
+    HalfIn<T, kRagged> hdy[2];
     uint4 codes[2];
     float scale[2], along = 0.f;
 #pragma unroll
@@ -256,20 +283,20 @@ __global__ void __launch_bounds__(512) rmsnorm_bwd32_kernel(const NormBwd a) {
       hdy[j].zero();
       codes[j] = make_uint4(0, 0, 0, 0);
       scale[j] = 0.f;
-      if (i >= a.d) continue;
-      hdy[j].load(static_cast<const T*>(a.dy) + r * a.dy_ld + i);
-      codes[j] = load_codes(a.codes + r * a.c_ld + i);
-      scale[j] = pow2_of(a.scales[r * a.s_ld + i / kGroup]) * rstd;
+      if (!kRagged && !at[j].live) continue;
+      hdy[j].load(py + r * a.dy_ld + i, at[j], extent_of(py, a.rows, a.dy_ld, a.d));
+      codes[j] = load_codes<kRagged>(a.codes + r * a.c_ld + i, at[j]);
+      if (at[j].live) scale[j] = pow2_of(a.scales[r * a.s_ld + i / kGroup]) * rstd;
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int64_t i = threadIdx.x * 16 + j * step;
-      if (i >= a.d) continue;
-      Half<T> hw;
-      hw.load_shared(static_cast<const T*>(a.w) + i);
+      if (!at[j].live) continue;
+      HalfIn<T, kRagged> hw;
+      hw.template load<true>(pw + i, at[j], in_w);
       float dy[16], xh[16], w[16];
-      hdy[j].get(dy);
-      hw.get(w);
+      hdy[j].get(dy, at[j]);
+      hw.get(w, at[j]);
       unpack_half(codes[j], scale[j], xh);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -281,141 +308,32 @@ __global__ void __launch_bounds__(512) rmsnorm_bwd32_kernel(const NormBwd a) {
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const int64_t i = threadIdx.x * 16 + j * step;
-      if (i >= a.d) continue;
-      Half<T> hw, hdh;
-      hw.load_shared(static_cast<const T*>(a.w) + i);
+      if (!kRagged && !at[j].live) continue;  // ragged rows are stored by whole warps
+      HalfIn<T, kRagged> hw, hdh;
+      hw.zero();
       hdh.zero();
-      if (a.dh) hdh.load(static_cast<const T*>(a.dh) + r * a.dh_ld + i);
+      if (kRagged || at[j].live) {
+        hw.template load<true>(pw + i, at[j], in_w);
+        if (a.dh) hdh.load(ph + r * a.dh_ld + i, at[j], extent_of(ph, a.rows, a.dh_ld, a.d));
+      }
       float dy[16], xh[16], w[16], dh[16];
-      hdy[j].get(dy);
-      hw.get(w);
-      hdh.get(dh);
+      hdy[j].get(dy, at[j]);
+      hw.get(w, at[j]);
+      hdh.get(dh, at[j]);
       unpack_half(codes[j], scale[j], xh);
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         dh[k] += rstd * (dy[k] * w[k] - xh[k] * along);
         xh[k] *= w[k];
       }
-      store_half(static_cast<T*>(a.dx) + r * a.dx_ld + i, dh);
-      if (a.y) store_half(static_cast<T*>(a.y) + r * a.y_ld + i, xh);
+      put_values<kRagged>(static_cast<T*>(a.dx) + r * a.dx_ld + i, dh, at[j]);
+      if (a.y) put_values<kRagged>(static_cast<T*>(a.y) + r * a.y_ld + i, xh, at[j]);
     }
   }
   if (!a.dw) return;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int64_t i = threadIdx.x * 16 + j * step;
-    if (i >= a.d) continue;
-#pragma unroll
-    for (int k = 0; k < 16; k += 4)
-      *reinterpret_cast<float4*>(a.part + (int64_t)blockIdx.x * a.d + i + k) =
-          make_float4(acc[j][k], acc[j][k + 1], acc[j][k + 2], acc[j][k + 3]);
-  }
-}
-
-// ---------------------------------------------------------------------------------------------
-// Unaligned rows: K values a thread, a row's threads apart.
-// ---------------------------------------------------------------------------------------------
-template <typename T, bool kWarpRows, int K>
-__global__ void __launch_bounds__(kWarpRows ? kThreads : 512) add_rmsnorm_pack_kernel(const NormFwd a) {
-  __shared__ float ws[32];
-  const int lane = threadIdx.x & 31, stride = kWarpRows ? 32 : blockDim.x, d = (int)a.d;
-  const int64_t r = kWarpRows ? (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
-  if (r >= a.rows) return;
-  const int i0 = kWarpRows ? lane : threadIdx.x;
-  const T *x = static_cast<const T*>(a.x) + r * a.x_ld, *add = static_cast<const T*>(a.a) + r * a.a_ld;
-  const T* w = static_cast<const T*>(a.w);
-  T *h = static_cast<T*>(a.h) + r * a.h_ld, *y = static_cast<T*>(a.y) + r * a.y_ld;
-  uint8_t *codes = a.codes + r * a.c_ld, *scales = a.scales + r * a.s_ld;
-  T vx[K], va[K];  // all loads before the first use
-#pragma unroll
-  for (int k = 0; k < K; ++k) vx[k] = i0 + k * stride < d ? x[i0 + k * stride] : from_float<T>(0.f);
-  if (a.a)
-#pragma unroll
-    for (int k = 0; k < K; ++k) va[k] = i0 + k * stride < d ? add[i0 + k * stride] : from_float<T>(0.f);
-  float v[K], ss = 0.f;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    v[k] = to_float(vx[k]);
-    if (a.a) v[k] = to_float(from_float<T>(v[k] + to_float(va[k])));
-    ss = fmaf(v[k], v[k], ss);
-  }
-  const float rstd = rstd_of(row_sum<kWarpRows>(ss, 32, ws), a);
-  if (i0 == 0) a.rstd[r] = rstd;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int i = i0 + k * stride;
-    if (i - lane >= d) break;  // whole warps: a group is a warp's 32 lanes
-    int s;
-    const uint32_t c = pack_lane(v[k], &s);
-    if (lane == 0) scales[i / kGroup] = (uint8_t)s;
-    if (i < d) {
-      codes[i] = (uint8_t)c;
-      if (a.h) h[i] = from_float<T>(v[k]);
-      y[i] = from_float<T>(v[k] * rstd * to_float(w[i]));
-    }
-  }
-}
-
-template <typename T, bool kWarpRows, int K>
-__global__ void __launch_bounds__(kWarpRows ? kThreads : 512) rmsnorm_bwd_kernel(const NormBwd a) {
-  __shared__ float ws[2][32];
-  __shared__ float col[kWarpRows ? kWarps : 1][kWarpRow];
-  const int lane = threadIdx.x & 31, stride = kWarpRows ? 32 : blockDim.x, d = (int)a.d;
-  const int i0 = kWarpRows ? lane : threadIdx.x;
-  const int64_t step = (int64_t)gridDim.x * (kWarpRows ? kWarps : 1);
-  int64_t r = kWarpRows ? (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
-  const T* w = static_cast<const T*>(a.w);
-  float acc[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) acc[k] = 0.f;
-  const float inv_d = 1.0f / (float)a.d;
-  for (int turn = 0; r < a.rows; r += step, ++turn) {
-    const float rstd = a.rstd[r];
-    const T *dy = static_cast<const T*>(a.dy) + r * a.dy_ld, *dh = static_cast<const T*>(a.dh) + r * a.dh_ld;
-    T *dx = static_cast<T*>(a.dx) + r * a.dx_ld, *y = static_cast<T*>(a.y) + r * a.y_ld;
-    const uint8_t *codes = a.codes + r * a.c_ld, *scales = a.scales + r * a.s_ld;
-    T vy[K], vh[K];  // all loads before the first use
-    uint8_t vc[K], vs[K];
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = i0 + k * stride;
-      vy[k] = i < d ? dy[i] : from_float<T>(0.f);
-      vc[k] = i < d ? codes[i] : (uint8_t)0;
-      vs[k] = i < d ? scales[i / kGroup] : (uint8_t)0;
-    }
-    if (a.dh)
-#pragma unroll
-      for (int k = 0; k < K; ++k) vh[k] = i0 + k * stride < d ? dh[i0 + k * stride] : from_float<T>(0.f);
-    float xh[K], along = 0.f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      xh[k] = unpack_one(vc[k], vs[k]) * rstd;
-      const float g = to_float(vy[k]), wi = i0 + k * stride < d ? to_float(w[i0 + k * stride]) : 0.f;
-      along = fmaf(g * wi, xh[k], along);
-      acc[k] = fmaf(g, xh[k], acc[k]);
-    }
-    along = row_sum<kWarpRows>(along, 32, ws[turn & 1]) * inv_d;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const int i = i0 + k * stride;
-      if (i < d) {
-        const float wi = to_float(w[i]);
-        float g = rstd * (to_float(vy[k]) * wi - xh[k] * along);
-        if (a.dh) g += to_float(vh[k]);
-        dx[i] = from_float<T>(g);
-        if (a.y) y[i] = from_float<T>(xh[k] * wi);
-      }
-    }
-  }
-  if (!a.dw) return;
-  float* part = a.part + (int64_t)blockIdx.x * a.d;
-  if (kWarpRows) {
-    warp_rows_part<K>(a, acc, part, col, i0, stride, true);
-  } else {
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      if (i0 + k * stride < d) part[i0 + k * stride] = acc[k];
-  }
+  for (int j = 0; j < 2; ++j)
+    put_part<kRagged>(a.part + (int64_t)blockIdx.x * a.d + threadIdx.x * 16 + j * step, acc[j], at[j].live);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -502,12 +420,12 @@ __global__ void __launch_bounds__(kSumWarps * 32) rmsnorm_dw_sum_kernel(const No
   static_cast<T*>(a.dw)[i] = from_float<T>(sum);
 }
 
-// Threads of a CTA: 16 values each (32 in rows over kLaneRow), eight warps where a warp holds rows.
+// Threads of a CTA: 16 values each (32 in rows over kHalfRow), eight warps where a warp holds rows.
 int threads_of(int64_t d) {
   if (d <= kWarpRow) return kThreads;
-  return (int)(d <= kLaneRow ? (d + 511) / 512 : (d + 1023) / 1024) * 32;
+  return (int)(d <= kHalfRow ? (d + 511) / 512 : (d + 1023) / 1024) * 32;
 }
-// Lanes of an aligned row of up to kWarpRow values: a power of two, two at least (a group).
+// Lanes of a row of up to kWarpRow values: a power of two, two at least (a group).
 int lanes_of(int64_t d) {
   int n = 2;
   while (n * 16 < d) n *= 2;
@@ -543,25 +461,26 @@ int gsa_add_rmsnorm_pack(int dtype, int64_t rows, int64_t d, const void* x, int6
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const int threads = threads_of(d);
-    const bool aligned = d % 16 == 0 && halves_ok<T>(x, x_ld) && (!a || halves_ok<T>(a, a_ld)) &&
-                         (!h || halves_ok<T>(h, h_ld)) && halves_ok<T>(y, y_ld) && halves_ok<T>(weight, 0);
-    const unsigned row_grid = (unsigned)rows, warp_grid = (unsigned)((rows + kWarps - 1) / kWarps);
-    if (aligned && d <= kWarpRow) {
-      const int64_t per = kWarps * (32 / lanes);
-      add_rmsnorm_pack16_kernel<T, true, 1, kThreads><<<(unsigned)((rows + per - 1) / per), kThreads, 0, s>>>(p);
-    } else if (aligned && d <= kLaneRow) {
-      add_rmsnorm_pack16_kernel<T, false, 1, 512><<<row_grid, threads, 0, s>>>(p);
-    } else if (aligned && d <= kMaxRow) {
-      add_rmsnorm_pack16_kernel<T, false, 2, 512><<<row_grid, threads, 0, s>>>(p);
-    } else if (d <= 128) {
-      add_rmsnorm_pack_kernel<T, true, 4><<<warp_grid, kThreads, 0, s>>>(p);
-    } else if (d <= kWarpRow) {
-      add_rmsnorm_pack_kernel<T, true, 16><<<warp_grid, kThreads, 0, s>>>(p);
-    } else if (d <= kLaneRow) {
-      add_rmsnorm_pack_kernel<T, false, 16><<<row_grid, threads, 0, s>>>(p);
-    } else {
-      add_rmsnorm_pack_long_kernel<T><<<row_grid, kThreads, 0, s>>>(p);
-    }
+    const bool whole = d % 16 == 0 && halves_ok<T>(x, x_ld) && (!a || halves_ok<T>(a, a_ld)) &&
+                       (!h || halves_ok<T>(h, h_ld)) && halves_ok<T>(y, y_ld) && halves_ok<T>(weight, 0);
+    auto go = [&](auto ragged) {
+      constexpr bool kRagged = decltype(ragged)::value;
+      const unsigned row_grid = (unsigned)rows;
+      if (d <= kWarpRow) {
+        const int64_t per = kWarps * (32 / lanes);
+        add_rmsnorm_pack16_kernel<T, kRagged, true, 1, kThreads>
+            <<<(unsigned)((rows + per - 1) / per), kThreads, 0, s>>>(p);
+      } else if (d <= kHalfRow) {
+        add_rmsnorm_pack16_kernel<T, kRagged, false, 1, 512><<<row_grid, threads, 0, s>>>(p);
+      } else if (d <= kMaxRow && kRagged) {  // 32 values a thread would leave one CTA an SM
+        add_rmsnorm_pack16_kernel<T, kRagged, false, 1, 1024><<<row_grid, (unsigned)((d + 511) / 512 * 32), 0, s>>>(p);
+      } else if (d <= kMaxRow) {
+        add_rmsnorm_pack16_kernel<T, false, false, 2, 512><<<row_grid, threads, 0, s>>>(p);
+      } else {
+        add_rmsnorm_pack_long_kernel<T><<<row_grid, kThreads, 0, s>>>(p);
+      }
+    };
+    whole ? go(std::false_type()) : go(std::true_type());
   });
   return launch_status();
 }
@@ -593,24 +512,23 @@ int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* 
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const int threads = threads_of(d);
-    const bool aligned = d % 16 == 0 && halves_ok<T>(dy, dy_ld) && (!dh || halves_ok<T>(dh, dh_ld)) &&
-                         halves_ok<T>(dx, dx_ld) && (!y || halves_ok<T>(y, y_ld)) && halves_ok<T>(weight, 0);
-    if (aligned && d <= kWarpRow) {
-      rmsnorm_bwd16_kernel<T, true><<<p.parts, kThreads, 0, s>>>(p);
-    } else if (aligned && d <= kLaneRow) {
-      rmsnorm_bwd16_kernel<T, false><<<p.parts, threads, 0, s>>>(p);
-    } else if (aligned && d <= kMaxRow) {
-      rmsnorm_bwd32_kernel<T><<<p.parts, threads, 0, s>>>(p);
-    } else if (d <= 128) {
-      rmsnorm_bwd_kernel<T, true, 4><<<p.parts, kThreads, 0, s>>>(p);
-    } else if (d <= kWarpRow) {
-      rmsnorm_bwd_kernel<T, true, 16><<<p.parts, kThreads, 0, s>>>(p);
-    } else if (d <= kLaneRow) {
-      rmsnorm_bwd_kernel<T, false, 16><<<p.parts, threads, 0, s>>>(p);
-    } else {
-      rmsnorm_bwd_long_kernel<T><<<(unsigned)rows, kThreads, 0, s>>>(p);
-      if (dw) rmsnorm_dw_part_kernel<T><<<dim3((unsigned)((d + kThreads - 1) / kThreads), p.parts), kThreads, 0, s>>>(p);
-    }
+    const bool whole = d % 16 == 0 && halves_ok<T>(dy, dy_ld) && (!dh || halves_ok<T>(dh, dh_ld)) &&
+                       halves_ok<T>(dx, dx_ld) && (!y || halves_ok<T>(y, y_ld)) && halves_ok<T>(weight, 0);
+    auto go = [&](auto ragged) {
+      constexpr bool kRagged = decltype(ragged)::value;
+      if (d <= kWarpRow) {
+        rmsnorm_bwd16_kernel<T, kRagged, true><<<p.parts, kThreads, 0, s>>>(p);
+      } else if (d <= kHalfRow) {
+        rmsnorm_bwd16_kernel<T, kRagged, false><<<p.parts, threads, 0, s>>>(p);
+      } else if (d <= kMaxRow) {
+        rmsnorm_bwd32_kernel<T, kRagged><<<p.parts, threads, 0, s>>>(p);
+      } else {
+        rmsnorm_bwd_long_kernel<T><<<(unsigned)rows, kThreads, 0, s>>>(p);
+        if (dw)
+          rmsnorm_dw_part_kernel<T><<<dim3((unsigned)((d + kThreads - 1) / kThreads), p.parts), kThreads, 0, s>>>(p);
+      }
+    };
+    whole ? go(std::false_type()) : go(std::true_type());
     if (dw) launch_chained(rmsnorm_dw_sum_kernel<T>, (unsigned)((d + 31) / 32), kSumWarps * 32, 0, s, p);
   });
   return launch_status();

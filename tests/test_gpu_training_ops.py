@@ -447,6 +447,85 @@ def test_norm_special_rows(cuda_ok):
 
 
 # -- loss ---------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [1, 2, 7, 15, 17, 31, 33, 95, 250, 511, 513, 1003, 8193, 16381])
+def test_rows_at_any_offset(cuda_ok, dtype, n):
+    """Rows that start at every offset within 32 bytes, NaN around them, give the bits of contiguous ones; outputs
+    with gaps between their rows leave the gaps, and what lies before and behind, as they were."""
+    import gsa_b200 as gsa
+    from gsa_b200 import _lib
+
+    ops, lib, rows, guard = gsa.ops, _lib.lib(), 3, 7777.0
+
+    def spread(t, off, gap):
+        """t's rows at that element offset and distance in storage of NaN."""
+        ld = t.shape[-1] + gap
+        v = torch.full((off + t.shape[0] * ld + 64,), math.nan, device=DEV, dtype=dtype).as_strided(t.shape, (ld, 1), off)
+        return v.copy_(t)
+
+    def holes(width, off, ld):
+        """An output for rows of that width, and what tells whether the rest of its storage is as it was."""
+        base = torch.full((off + rows * ld + 64,), guard, device=DEV, dtype=dtype)
+        out = base.as_strided((rows, width), (ld, 1), off)
+        return out, lambda: bool((base.as_strided((rows, ld - width), (ld, 1), off + width) == guard).all()) and bool(
+            (base[:off] == guard).all()) and bool((base[off + rows * ld:] == guard).all())
+
+    x, a, dh = (_randn(i, rows, n, dtype=dtype) for i in (1, 2, 3))
+    gu, w = _randn(4, rows, 2 * n, dtype=dtype), _randn(5, 1, n, dtype=dtype)
+    want_p = ops.pack_e4m3(x)
+    want_x = ops.unpack_e4m3(want_p)
+    want_z, pgu = ops.silu_mul_packed(gu)
+    want_dgu, want_z2 = ops.silu_mul_packed_backward(x, pgu, want_z=True)
+    want_h, want_y, ph, rstd = ops.add_rmsnorm_packed(x, a, w[0], 1e-5)
+    want_dx, want_dw, want_y2 = ops.rmsnorm_packed_backward(x, ph, rstd, w[0], dh=dh, want_y=True)
+    t = _lib.DTYPE_BF16 if dtype is torch.bfloat16 else _lib.DTYPE_F32
+    stream = torch.cuda.current_stream().cuda_stream
+    c_ld, s_ld = (n + 15) // 16 * 16, (n + 31) // 32
+    for off in range(32 // x.element_size()):
+        xs, as_, dhs, gus, ws = (spread(v, off, gap) for v, gap in ((x, 3), (a, 1), (dh, 2), (gu, 5), (w, 0)))
+        p = ops.pack_e4m3(xs)
+        assert torch.equal(p.scales, want_p.scales)
+        assert torch.equal(p.codes.view(torch.uint8)[:, :n], want_p.codes.view(torch.uint8)[:, :n])
+        z, q = ops.silu_mul_packed(gus)
+        assert torch.equal(z, want_z) and torch.equal(q.unpack(), pgu.unpack())
+        dgu, z = ops.silu_mul_packed_backward(xs, pgu, want_z=True)
+        assert torch.equal(dgu, want_dgu) and torch.equal(z, want_z2)
+        h, y, q, r = ops.add_rmsnorm_packed(xs, as_, ws[0], 1e-5)
+        assert torch.equal(h, want_h) and torch.equal(y, want_y) and torch.equal(q.unpack(), ph.unpack())
+        assert torch.equal(r, rstd)
+        dx, dw, y = ops.rmsnorm_packed_backward(xs, ph, rstd, ws[0], dh=dhs, want_y=True)
+        assert torch.equal(dx, want_dx) and torch.equal(dw, want_dw) and torch.equal(y, want_y2)
+        # outputs at that offset, by the C entries
+        ld = n + 5
+        out, kept = holes(n, off, ld)
+        codes, scales = want_p.codes.data_ptr(), want_p.scales.data_ptr()
+        assert lib.gsa_unpack_e4m3(t, rows, n, codes, c_ld, scales, s_ld, out.data_ptr(), ld, stream) == 0
+        assert torch.equal(out, want_x) and kept()
+        out, kept = holes(n, off, ld)
+        q = gsa.PackedActivation.empty((rows, 2, n), dtype, DEV)
+        qc, qs = q.codes.data_ptr(), q.scales.data_ptr()
+        assert lib.gsa_silu_mul_pack(t, rows, n, gu.data_ptr(), 2 * n, out.data_ptr(), ld, qc, c_ld, qs, s_ld, stream) == 0
+        assert torch.equal(out, want_z) and torch.equal(q.unpack(), pgu.unpack()) and kept()
+        out, kept = holes(2 * n, off, ld + n)
+        out2, kept2 = holes(n, off, ld)
+        assert lib.gsa_silu_mul_packed_backward(t, rows, n, x.data_ptr(), n, pgu.codes.data_ptr(), c_ld, pgu.scales.data_ptr(),
+                                                s_ld, out.data_ptr(), ld + n, out2.data_ptr(), ld, stream) == 0
+        assert torch.equal(out.reshape(want_dgu.shape), want_dgu) and torch.equal(out2, want_z2) and kept() and kept2()
+        out, kept = holes(n, off, ld)
+        out2, kept2 = holes(n, off, ld)
+        q, r = gsa.PackedActivation.empty((rows, n), dtype, DEV), torch.empty(rows, device=DEV)
+        assert lib.gsa_add_rmsnorm_pack(t, rows, n, x.data_ptr(), n, a.data_ptr(), n, w.data_ptr(), 1e-5, out.data_ptr(), ld,
+                                        out2.data_ptr(), ld, q.codes.data_ptr(), c_ld, q.scales.data_ptr(), s_ld,
+                                        r.data_ptr(), stream) == 0
+        assert torch.equal(out, want_h) and torch.equal(out2, want_y) and torch.equal(r, rstd) and kept() and kept2()
+        out, kept = holes(n, off, ld)
+        out2, kept2 = holes(n, off, ld)
+        assert lib.gsa_rmsnorm_packed_backward(t, rows, n, x.data_ptr(), n, dh.data_ptr(), n, w.data_ptr(), ph.codes.data_ptr(),
+                                               c_ld, ph.scales.data_ptr(), s_ld, rstd.data_ptr(), out.data_ptr(), ld,
+                                               out2.data_ptr(), ld, None, None, 0, stream) == 0
+        assert torch.equal(out, want_dx) and torch.equal(out2, want_y2) and kept() and kept2()
+
+
 def _loss_oracle(logits, labels, ignore=-100):
     x = logits.double()[:, :-1]
     t = labels[:, 1:]
