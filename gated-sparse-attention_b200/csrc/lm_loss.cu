@@ -4,7 +4,7 @@
 //   loss = mean over the counted positions of (log sum_v e^{x_v} - x_target)
 //   grad = (softmax(x) - onehot(target)) / count, zero in the rows that do not count
 //
-// A CTA takes a row (a warp one of up to 4 KB, eight lanes one of up to 1 KB): its maximum and sum in one pass (online), then the gradient
+// A CTA takes a row (a warp one of up to 4 KB, two to eight lanes one of up to 1 KB): its maximum and sum in one pass (online), then the gradient
 // from a second reading, which registers serve for short rows and the L2 for long ones: the rows in flight are up to
 // 76 MB.  So HBM sees each logit about once (1.1 times for rows of 250 KB) and each gradient value once.
 // Exponentials are 2^(x log2 e - M) by one multiply-add (two values an instruction) and one ex2, M the rounded m log2 e:
@@ -477,12 +477,16 @@ cudaError_t launch_rows(const LossArgs& a, int* grid, cudaStream_t s) {
 // Threads a row: 1024 threads an SM in any case, on as many rows as their second reading finds in L2 -- 16 rows an SM of
 // up to 20 KB (48 MB in flight), 8 of up to 48 KB, 4 of up to 112 KB, 2 of up to 320 KB, then 1.  Measured in TB/s with
 // twice the threads a row | as here | with half: 8 KB rows 4.1 | 4.6 | -, 40 KB 4.8 | 5.1 | 4.6, 98 KB 4.6 | 4.8 | 4.4,
-// 250 KB 4.9 | 5.0 | 4.4, 501 KB (fp32) - | 5.1 | 4.5.
+// 250 KB 4.9 | 5.0 | 4.4, 501 KB (fp32) - | 5.1 | 4.5.  Short rows take lanes of a warp, with four pieces of 16 bytes in
+// flight (eight spill; us here | with eight lanes, or a warp over 1 KB, and eight pieces: 131,072 x 16 bf16 12 | 31, 71,652 x 52 fp32
+// 13 | 21, 65,536 x 384 fp32 47 | 63, 131,072 x 333 bf16 57 | 57).
 template <typename T>
 cudaError_t launch_loss(const LossArgs& a, int* grid, cudaStream_t s) {
   const int64_t bytes = a.V * (int64_t)sizeof(T);
-  if (bytes <= 1024) return launch_rows<T, 8, 256, 4, 8>(a, grid, s);
-  if (bytes <= 4096) return launch_rows<T, 32, 256, 4, 8>(a, grid, s);
+  if (bytes <= 64) return launch_rows<T, 2, 256, 4, 2>(a, grid, s);
+  if (bytes <= 256) return launch_rows<T, 4, 256, 4, 4>(a, grid, s);
+  if (bytes <= 1024) return launch_rows<T, 8, 256, 4, 4>(a, grid, s);
+  if (bytes <= 4096) return launch_rows<T, 32, 256, 4, 4>(a, grid, s);
   if (bytes <= 20 << 10) return launch_rows<T, 64, 64, 16, 6>(a, grid, s);
   if (bytes <= 48 << 10) return launch_rows<T, 128, 128, 8, 6>(a, grid, s);
   if (bytes <= 112 << 10) return launch_rows<T, 256, 256, 4, 6>(a, grid, s);

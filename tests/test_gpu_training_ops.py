@@ -545,7 +545,7 @@ def _loss_oracle(logits, labels, ignore=-100):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("B,L,V", [(1, 2, 1), (1, 2, 2), (2, 96, 384), (3, 17, 1000), (1, 33, 4097), (2, 5, 128256), (1, 600, 31),
+@pytest.mark.parametrize("B,L,V", [(1, 2, 1), (1, 2, 2), (3, 700, 9), (2, 300, 64), (1, 50, 257), (4, 9, 2047), (2, 96, 384), (3, 17, 1000), (1, 33, 4097), (2, 5, 128256), (1, 600, 31),
                                    (1, 3, 32768), (700, 2, 8), (1, 9, 50257), (2, 200, 32768), (1, 3, 20000),
                                    (1, 150, 65544), (1, 3, 131072), (1, 2, 262152)])
 def test_loss_and_gradient(cuda_ok, dtype, B, L, V):
@@ -583,7 +583,7 @@ def test_loss_gradient_is_that_of_differences(cuda_ok):
     assert abs(float((grad.double() * v).sum() - (up - down) / (2 * e))) < 400 * 16 * U
 
 
-@pytest.mark.parametrize("V", [70, 3000, 4099, 32768, 65536, 128256])
+@pytest.mark.parametrize("V", [70, 500, 3000, 4099, 32768, 65536, 128256])
 def test_loss_special_rows(cuda_ok, V):
     """Masked (-inf) logits, a target among them, large and equal logits, rows that do not count, no row that counts, another
     ignore_index, a label out of range, NaN."""
@@ -648,6 +648,45 @@ def test_loss_special_rows(cuda_ok, V):
     wrong[0, 2] = 12345678
     loss, _ = ops.next_token_loss(x, wrong, ignore_index=12345678)
     assert bool(torch.isfinite(loss))
+    ops.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [3, 8, 16, 31, 60, 64, 100])
+def test_loss_special_short_rows(cuda_ok, dtype, V):
+    """Rows that two to eight lanes hold, special ones beside ordinary ones in a warp."""
+    from gsa_b200 import _lib, ops
+
+    L = 40
+    x = _randn(1, 1, L, V, dtype=dtype)
+    x[0, 1, 1:] = -math.inf
+    x[0, 4] = torch.finfo(dtype).min
+    x[0, 9, 0] = -math.inf
+    x[0, 17] = 500.0
+    labels = torch.randint(0, V, (1, L), device=DEV, generator=_gen(2))
+    labels[0, 2] = labels[0, 5] = 0
+    labels[0, 10] = V - 1
+    labels[0, 20:23] = -100
+    want, g, size, far, _ = _loss_oracle(x, labels)
+    plain = x.clone()
+    plain[0, 4] = 0.0  # its loss is log V too, which the value's size does not enter
+    loss_size = _loss_oracle(plain, labels)[-1]
+    loss, grad = ops.next_token_loss(x, labels)
+    # two lanes at least: V / 2 additions after one another, and 2^(x log2 e - M) as above
+    _near(loss, want, (V / 2 + 256) * U * (1 + loss_size))
+    _near(grad, g, size * (V / 2 + 256) * U)
+    assert bool((grad[0, 19:22] == 0).all()) and bool((grad[0, -1] == 0).all()) and bool((grad[0, 1, 1:] == 0).all())
+    # a row without any probability, a NaN and labels out of range make their rows NaN, and no other
+    y, bad = x.clone(), labels.clone()
+    y[0, 6] = -math.inf
+    y[0, 11, V // 2] = math.nan
+    bad[0, 31], bad[0, 33] = V, -1
+    loss, other = ops.next_token_loss(y, bad)
+    assert math.isnan(float(loss))
+    for t in range(L):
+        assert bool(torch.isnan(other[0, t]).all()) if t in (6, 11, 30, 32) else torch.equal(other[0, t], grad[0, t]), t
+    with pytest.raises(_lib.GSAError):
+        ops.check_device_error()
     ops.check_device_error()
 
 
