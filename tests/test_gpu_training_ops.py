@@ -56,6 +56,8 @@ ROTARY = [
     (1, 1, 1, 1, 2, 2, False),
     (64, 1, 32, 8, 128, 128, False),
     (2, 77, 8, 2, 64, 64, False),
+    (2, 19, 6, 2, 80, 40, False),
+    (2, 300, 4, 1, 96, 24, True),
     (2, 33, 32, 8, 128, 64, True),
     (3, 19, 9, 3, 80, 80, False),
     (3, 19, 9, 3, 80, 20, True),
