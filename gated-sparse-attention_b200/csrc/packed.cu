@@ -8,7 +8,10 @@
 //
 // Products are in 32 bits; an output is rounded once, to its type.  All are bound by the bytes that they move, so
 // a thread holds 16 neighbouring values (half a group, 32-byte loads and stores, one shuffle for the scale); where rows are
-// not whole multiples of that, or not aligned, through 16-byte pieces (kRagged: packed.cuh).
+// not whole multiples of that, or not aligned, through aligned pieces (kRagged: packed.cuh).  Whole rows run at HBM's rate (of
+// 6.55 TB/s for a copy): pack and unpack of 32768 x 4096 bf16 128 us, 6.4 TB/s; SwiGLU and its backward pass of 16384 x
+// 11008 0.50 ms, 6.5 TB/s.  Ragged ones are bound by instructions: 32768 x 4090 bf16 155 us (5.2 TB/s) and 0.53 ms (4.5); fp32
+// 16384 x 4090 124 us and 0.34 ms (5.4, 6.3).
 #include <algorithm>
 
 #include "packed.cuh"
@@ -60,7 +63,8 @@ __device__ __forceinline__ Place place_of(const Cut& c, int skip = 0, int each =
   return {r, i, spot_of<kRagged>(i, c.n, e < c.halves)};
 }
 
-// Two halves a thread, both loaded first: one alone leaves too little in flight for HBM.
+// Two halves a thread, both loaded first: one alone leaves too little in flight for HBM (69 us, 65 with two, for 32768 x
+// 4096 bf16).
 constexpr int kPackEach = 2;
 
 template <typename T, bool kRagged>
@@ -139,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, kRagged && sizeof(T) == 4 ? 3 : 4)
 }
 
 template <typename T, bool kRagged>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 ? 4 : 3)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 2 && !kRagged ? 4 : 3)
     silu_mul_bwd16_kernel(const Cut c, const T* dz, int64_t dz_ld, const uint8_t* codes, int64_t c_ld,
                           const uint8_t* scales, int64_t s_ld, T* dgu, int64_t dgu_ld, T* z, int64_t z_ld) {
   const Place p = place_of<kRagged>(c);
