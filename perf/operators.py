@@ -274,19 +274,12 @@ _PLAIN = {"rotary": _rotary, "pack": _pack, "swiglu": _swiglu, "norm": _norm, "l
 
 
 # -- the framework's calls ----------------------------------------------------------------------
-_gsa = None
-
-
 def _package():
-    """The package, imported by the first call, as a user's program imports it once."""
-    global _gsa
-    if _gsa is None:
-        at = str(Path.cwd() / "gated-sparse-attention_b200")
-        if at not in sys.path:
-            sys.path.insert(0, at)
-        import gsa_b200
-        _gsa = gsa_b200
-    return _gsa
+    at = str(Path.cwd() / "gated-sparse-attention_b200")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import gsa_b200
+    return gsa_b200
 
 
 def _own(s):
