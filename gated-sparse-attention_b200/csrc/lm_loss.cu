@@ -8,9 +8,11 @@
 // from a second reading, which registers serve for short rows and the L2 for long ones: the rows in flight are up to
 // 76 MB.  So HBM sees each logit about once (1.1 times for rows of 250 KB) and each gradient value once.
 // Exponentials are 2^(x log2 e - M) by one multiply-add (two values an instruction) and one ex2, M the rounded m log2 e:
-// M is what the sums and the gradient share, so its rounding cancels.  Values under kLow, where that would overflow,
-// weigh 0 beside any other; a row that has nothing else (masked throughout with the type's lowest value, or with
-// -inf) is taken by differences first.  Sums are in 32 bits within a row and in 64 across rows; each CTA adds its
+// M is what the sums and the gradient share, so its rounding, a factor 2^r on all of them, cancels as long as 2^r does not
+// leave the range: |r| is half a step of M, 4 up to kFar.  A row whose |M| is larger (masked throughout with any value or
+// with -inf, or with a far largest one) is taken by differences first; beside a largest value within kFar, values under
+// kLow weigh 0 and are not met at all (a thread that has seen nothing else would be left with an r of its own of
+// any size).  Sums are in 32 bits within a row and in 64 across rows; each CTA adds its
 // rows in order and one CTA adds the CTAs' sums in order, so a loss is the same bits every time.  8192 x 128256 bf16: 0.70 to
 // 0.82 ms on different machines, 5.1 to 6.0 TB/s; what keeps it from a copy's 6.55 is latency between the two passes of a row
 // (no unit is more than two thirds busy).
@@ -28,7 +30,8 @@ constexpr int kCounters = 64;         // CTAs of the count kernel
 constexpr int64_t kSelfCount = 2048;  // labels up to which every CTA counts for itself
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLn2 = 0.693147181f;
-constexpr float kLow = -1e38f;
+constexpr float kFar = 0x1p27f;   // of M
+constexpr float kLow = -0x1p28f;  // of a logit: 1.7e8 under any largest value within kFar; |r| <= 16 down to there
 
 struct Workspace {
   double sums[kMaxGrid];      // of each CTA's rows
@@ -282,11 +285,9 @@ __device__ __forceinline__ float row_reduce(float v, float* ws) {
   return v;
 }
 
-// A row with no value above kLow, by differences first, a value at a time; the gradient of its values i0 .. i1 - 1.  Rows
-// of -inf alone come out NaN.
+// A row of |M| past kFar, by differences first, a value at a time.  Rows with a NaN or a +inf, or of -inf alone, come out NaN.
 template <typename T, int kRow>
-__device__ __noinline__ float low_row(const T* x, T* g, int V, int i0, int i1, int target, int lane, float inv_count,
-                                      float* ws) {
+__device__ __noinline__ float far_row(const T* x, T* g, int V, int target, int lane, float inv_count, float* ws) {
   if (kRow > 32) __syncthreads();  // ws has been read
   float m = -INFINITY, s = 0.f;
   for (int i = lane; i < V; i += kRow) m = fmaxf(m, to_float(x[i]));
@@ -294,7 +295,7 @@ __device__ __noinline__ float low_row(const T* x, T* g, int V, int i0, int i1, i
   for (int i = lane; i < V; i += kRow) s += expf(to_float(x[i]) - m);
   s = row_reduce<kRow, false>(s, ws);
   if (g)
-    for (int i = i0 + lane; i < i1; i += kRow)
+    for (int i = lane; i < V; i += kRow)
       g[i] = from_float<T>(expf(to_float(x[i]) - m) * (inv_count / s) - (i == target ? inv_count : 0.f));
   return logf(s) - (to_float(x[target]) - m);
 }
@@ -371,10 +372,10 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
   }
   p = join_row<kRow>(p, ws);
   const float m = p.m, s = p.s;
-  if (m == -INFINITY && s == 0.f && !bad)
-    return low_row<T, kRow>(x, g, walk.V, 0, walk.V, (int)target, lane, inv_count, &ws[0].m);
-  // a label out of range, a NaN or a logit of +inf: the row's loss and gradient are NaN
-  const float loss = bad || m == INFINITY ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
+  if (!(fabsf(m) < kFar) && !bad)
+    return far_row<T, kRow>(x, g, walk.V, (int)target, lane, inv_count, &ws[0].m);
+  // a label out of range or a NaN: the row's loss and gradient are NaN
+  const float loss = bad ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
   if (!g) return loss;
   const float inv = isnan(loss) ? loss : inv_count / s;
   const int at = bad ? -1 : (int)target - walk.first;  // among the pieces' values
