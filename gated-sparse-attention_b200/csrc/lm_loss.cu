@@ -287,7 +287,7 @@ __device__ __forceinline__ float row_reduce(float v, float* ws) {
 
 // A row of |M| past kFar, by differences first, a value at a time.  Rows with a NaN or a +inf, or of -inf alone, come out NaN.
 template <typename T, int kRow>
-__device__ __noinline__ float far_row(const T* x, T* g, int V, int target, int lane, float inv_count, float* ws) {
+__device__ __noinline__ double far_row(const T* x, T* g, int V, int target, int lane, float inv_count, float* ws) {
   if (kRow > 32) __syncthreads();  // ws has been read
   float m = -INFINITY, s = 0.f;
   for (int i = lane; i < V; i += kRow) m = fmaxf(m, to_float(x[i]));
@@ -297,13 +297,13 @@ __device__ __noinline__ float far_row(const T* x, T* g, int V, int target, int l
   if (g)
     for (int i = lane; i < V; i += kRow)
       g[i] = from_float<T>(expf(to_float(x[i]) - m) * (inv_count / s) - (i == target ? inv_count : 0.f));
-  return logf(s) - (to_float(x[target]) - m);
+  return (double)logf(s) - ((double)to_float(x[target]) - (double)m);
 }
 
 // A row by kRow threads (neighbouring lanes, or the CTA); lane: the thread's number among them.  Returns the row's loss.
 template <typename T, int kRow, int kAhead>
-__device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
-                                          Part* ws) {
+__device__ __forceinline__ double row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
+                                           Part* ws) {
   constexpr int n = Piece<T>::n;
   const Position pos = position_of(a, r);
   const T* x = static_cast<const T*>(a.logits) + pos.b * a.xb + pos.t * a.xl;
@@ -316,7 +316,7 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
       for (int i = lane; i < walk.pieces; i += kRow) __stcs(gp + i, make_uint4(0, 0, 0, 0));
       for (int e = lane; e < walk.edges; e += kRow) g[walk.edge(e)] = from_float<T>(0.f);
     }
-    return 0.f;
+    return 0;
   }
   const float nan = __int_as_float(0x7fc00000);
   const bool bad = target < 0 || target >= a.V;
@@ -375,9 +375,11 @@ __device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t 
   if (!(fabsf(m) < kFar) && !bad)
     return far_row<T, kRow>(x, g, walk.V, (int)target, lane, inv_count, &ws[0].m);
   // a label out of range or a NaN: the row's loss and gradient are NaN
-  const float loss = bad ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
+  double loss = bad ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
+  const float inv = isnan(loss) ? nan : inv_count / s;
+  // x_target log2 e may leave the range of 32 bits where the loss does not
+  if (loss == INFINITY) loss = ((double)log2f(s) - ((double)x_target * kLog2e - m)) * kLn2;
   if (!g) return loss;
-  const float inv = isnan(loss) ? loss : inv_count / s;
   const int at = bad ? -1 : (int)target - walk.first;  // among the pieces' values
   const uint64_t neg_m = pair_of(-m, -m), inv2 = pair_of(inv, inv);
   for (int i0 = lane; i0 < walk.pieces; i0 += kAhead * kRow) {

@@ -1,5 +1,5 @@
 """The next-token loss over the whole range of its logits' type: rows whose largest value is far from zero, masks of any
-finite size beside ordinary logits.
+finite size beside ordinary logits, labels on masked values.
 
 Every row is also a call of its own, so that the mean hides nothing.  The oracle is the definition in 64 bits."""
 
@@ -108,3 +108,33 @@ def test_loss_masks_of_any_size(cuda_ok, dtype, nbytes):
             rows.append(row)
             labels.append(int(keep.nonzero()[0]))
     _check_rows(rows, labels)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("nbytes", BYTES)
+def test_loss_of_labels_far_below(cuda_ok, dtype, nbytes):
+    """The label's own logit masked with a finite value: the loss is its distance, as far as fp32 holds it, and also where
+    the mean over several rows does."""
+    from gsa_b200 import ops
+
+    V = nbytes * 8 // torch.finfo(dtype).bits
+    low = torch.finfo(dtype).min
+    rows, labels = [], []
+    for v in (-1e9, -1e10, -1e30, -2.3e38, -2.4e38, -3e38, low):
+        row = _ordinary(len(rows), V, dtype)
+        row[V // 2] = v
+        rows.append(row)
+        labels.append(V // 2)
+    for v, other in ((1e10, -1e10), (1e38, -1e38), (1.5e38, -1.5e38), (low, low)):
+        row = torch.full((V,), v, device=DEV).to(dtype)
+        row[V // 2] = other
+        rows.append(row)
+        labels.append(V // 2)
+    _check_rows(rows, labels)
+    # a row's loss past fp32's largest, and a mean that is not
+    x = torch.zeros(1, 6, V, device=DEV, dtype=dtype)
+    x[0, 2, 0], x[0, 2, 1] = -low, low
+    lab = torch.tensor([[0, 0, 0, 1, 0, 0]], device=DEV)
+    loss, grad = ops.next_token_loss(x, lab)
+    want = (-2 * low + 4 * math.log(V)) / 5
+    assert math.isfinite(float(loss)) and abs(float(loss) - want) <= 4 * U * want and bool(torch.isfinite(grad).all())
