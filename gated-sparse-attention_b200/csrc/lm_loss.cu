@@ -300,10 +300,16 @@ __device__ __noinline__ double far_row(const T* x, T* g, int V, int target, int 
   return (double)logf(s) - ((double)to_float(x[target]) - (double)m);
 }
 
-// A row by kRow threads (neighbouring lanes, or the CTA); lane: the thread's number among them.  Returns the row's loss.
+// The loss of a label far below the row's largest, in 64 bits (kept out of line: the registers of the usual case).
+__device__ __noinline__ double far_label(float s, float m, float x_target) {
+  return ((double)log2f(s) - ((double)x_target * kLog2e - m)) * kLn2;
+}
+
+// A row by kRow threads (neighbouring lanes, or the CTA); lane: the thread's number among them.  Returns the row's loss, or
+// adds one that 32 bits may not hold to far.
 template <typename T, int kRow, int kAhead>
-__device__ __forceinline__ double row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
-                                           Part* ws) {
+__device__ __forceinline__ float row_loss(const LossArgs& a, int64_t r, int64_t target, int lane, float inv_count,
+                                          Part* ws, double& far) {
   constexpr int n = Piece<T>::n;
   const Position pos = position_of(a, r);
   const T* x = static_cast<const T*>(a.logits) + pos.b * a.xb + pos.t * a.xl;
@@ -316,7 +322,7 @@ __device__ __forceinline__ double row_loss(const LossArgs& a, int64_t r, int64_t
       for (int i = lane; i < walk.pieces; i += kRow) __stcs(gp + i, make_uint4(0, 0, 0, 0));
       for (int e = lane; e < walk.edges; e += kRow) g[walk.edge(e)] = from_float<T>(0.f);
     }
-    return 0;
+    return 0.f;
   }
   const float nan = __int_as_float(0x7fc00000);
   const bool bad = target < 0 || target >= a.V;
@@ -372,14 +378,18 @@ __device__ __forceinline__ double row_loss(const LossArgs& a, int64_t r, int64_t
   }
   p = join_row<kRow>(p, ws);
   const float m = p.m, s = p.s;
-  if (!(fabsf(m) < kFar) && !bad)
-    return far_row<T, kRow>(x, g, walk.V, (int)target, lane, inv_count, &ws[0].m);
+  if (!(fabsf(m) < kFar) && !bad) {
+    far += far_row<T, kRow>(x, g, walk.V, (int)target, lane, inv_count, &ws[0].m);
+    return 0.f;
+  }
   // a label out of range or a NaN: the row's loss and gradient are NaN
-  double loss = bad ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
-  const float inv = isnan(loss) ? nan : inv_count / s;
-  // x_target log2 e may leave the range of 32 bits where the loss does not
-  if (loss == INFINITY) loss = ((double)log2f(s) - ((double)x_target * kLog2e - m)) * kLn2;
+  float loss = bad ? nan : (log2f(s) - fmaf(x_target, kLog2e, -m)) * kLn2;
+  if (loss == INFINITY) {  // x_target log2 e may leave the range of 32 bits where the loss does not
+    far += far_label(s, m, x_target);
+    loss = 0.f;
+  }
   if (!g) return loss;
+  const float inv = isnan(loss) ? loss : inv_count / s;
   const int at = bad ? -1 : (int)target - walk.first;  // among the pieces' values
   const uint64_t neg_m = pair_of(-m, -m), inv2 = pair_of(inv, inv);
   for (int i0 = lane; i0 < walk.pieces; i0 += kAhead * kRow) {
@@ -434,7 +444,8 @@ __global__ void __launch_bounds__(kCta, kCtas) lm_loss_kernel(const LossArgs a) 
   // two of row_ws in turn: a row's barrier is what frees the one before it
   for (int turn = 0; r < rows; r += step) {
     const int64_t next = target_of(a, r + step);
-    sum += row_loss<T, kRow, kAhead>(a, r, target, threadIdx.x % kRow, inv_count, row_ws[turn]);
+    const float loss = row_loss<T, kRow, kAhead>(a, r, target, threadIdx.x % kRow, inv_count, row_ws[turn], sum);
+    sum += loss;
     if (target != a.ignore) turn ^= 1;
     target = next;
   }
