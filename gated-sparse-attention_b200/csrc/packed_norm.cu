@@ -515,6 +515,7 @@ int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* 
   const NormBwd p{rows, d,    dy, dh, weight, dy_ld, dh_ld, codes, scales, c_ld,
                   s_ld, rstd, dx, y,  dw,     dx_ld, y_ld,  static_cast<float*>(workspace), parts_of(rows, d),
                   lanes_of(std::min<int64_t>(d, kWarpRow))};
+  int status = GSA_OK;
   typed(dtype, [&](auto e) {
     using T = decltype(e);
     const int threads = threads_of(d);
@@ -535,9 +536,12 @@ int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* 
       }
     };
     whole ? go(std::false_type()) : go(std::true_type());
-    if (dw) launch_chained(rmsnorm_dw_sum_kernel<T>, (unsigned)((d + 31) / 32), kSumWarps * 32, 0, s, p);
+    status = launch_status();
+    if (status == GSA_OK && dw &&
+        launch_chained(rmsnorm_dw_sum_kernel<T>, (unsigned)((d + 31) / 32), kSumWarps * 32, 0, s, p) != cudaSuccess)
+      status = GSA_ERR_LAUNCH;
   });
-  return launch_status();
+  return status;
 }
 
 }  // extern "C"
