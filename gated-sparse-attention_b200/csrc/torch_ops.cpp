@@ -10,6 +10,8 @@
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <functional>
+#include <numeric>
 #include <optional>
 #include <tuple>
 #include <vector>
@@ -261,6 +263,65 @@ bool separate(const Tensor& t) {
   return true;
 }
 
+// Whether a and b, of one element size, have a byte in common; true too where that cannot be told in a few thousand steps.
+// Elements at a + sum i_d s_d and b + sum j_d t_d meet where a bounded sum of the strides is the distance: one stride
+// after another from the largest, each multiple from which the rest can still make up what is left.
+bool overlap(const Tensor& a, const Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto extent = [](const Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += t.stride(i) * (t.size(i) - 1);
+    return (last + 1) * (int64_t)t.element_size();
+  };
+  const int64_t size = (int64_t)a.element_size();
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  if (bytes >= extent(a) || -bytes >= extent(b)) return false;
+  if (bytes % size) return true;
+  struct Term {
+    int64_t stride, lo, hi;  // any multiple from lo to hi
+  };
+  std::vector<Term> terms;
+  const auto add = [&](const Tensor& t, int64_t sign) {
+    for (int64_t i = 0; i < t.dim(); ++i) {
+      const int64_t stride = t.stride(i), last = t.size(i) - 1;
+      if (stride == 0 || last == 0) continue;
+      auto at = std::find_if(terms.begin(), terms.end(), [&](const Term& m) { return m.stride == stride; });
+      if (at == terms.end()) at = terms.insert(at, {stride, 0, 0});
+      (sign > 0 ? at->hi : at->lo) += sign * last;
+    }
+  };
+  add(a, 1);
+  add(b, -1);
+  std::sort(terms.begin(), terms.end(), [](const Term& x, const Term& y) { return x.stride > y.stride; });
+  const size_t n = terms.size();
+  std::vector<int64_t> least(n + 1, 0), most(n + 1, 0), unit(n + 1, 0);  // what the terms from i on can make up; their divisor
+  for (size_t i = n; i-- > 0;) {
+    least[i] = least[i + 1] + terms[i].lo * terms[i].stride;
+    most[i] = most[i + 1] + terms[i].hi * terms[i].stride;
+    unit[i] = std::gcd(unit[i + 1], terms[i].stride);
+  }
+  const auto floor_div = [](int64_t x, int64_t y) { return x / y - (x % y < 0); };
+  int steps = 1 << 14;
+  const std::function<bool(size_t, int64_t)> meet = [&](size_t i, int64_t left) {
+    if (i == n) return left == 0;
+    if (left % unit[i]) return false;
+    const int64_t s = terms[i].stride;
+    const int64_t lo = std::max(terms[i].lo, -floor_div(most[i + 1] - left, s)), hi = std::min(terms[i].hi, floor_div(left - least[i + 1], s));
+    for (int64_t c = lo; c <= hi; ++c)
+      if (--steps < 0 || meet(i + 1, left - c * s)) return true;
+    return false;
+  };
+  return meet(0, bytes / size);
+}
+
+// The same elements in the same places.
+bool same_place(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
 gsa_rotary_side side_of(const Tensor& x, const Tensor& out) {
   return {ptr(x), ptr(out), (int32_t)x.size(2), x.stride(0), x.stride(1), x.stride(2), out.stride(0), out.stride(1),
           out.stride(2)};
@@ -355,6 +416,15 @@ Pair rotary(const Tensor& q, const optional<Tensor>& k, const Tensor& positions,
       TORCH_CHECK_VALUE(o.sizes() == x.sizes() && (o.size(3) <= 1 || o.stride(3) == 1) && (o.is_contiguous() || separate(o)),
                         "rotary: out tensors have their inputs' shape, contiguous values and no two elements in one place");
     }
+    // the kernel reads an input (unless it is laid out anew first) while others of its CTAs write; an output that is its input
+    // itself is read and written by the same threads
+    for (int i = 0; i < (k ? 2 : 1); ++i)
+      for (int j = 0; j < (k ? 2 : 1); ++j) {
+        const Tensor &o = i ? *k_out : q_out, &x = j ? *k : q;
+        TORCH_CHECK_VALUE(x.stride(3) != 1 || (i == j && same_place(o, x)) || !overlap(o, x),
+                          "rotary: an out tensor overlaps an input without being that input's own place");
+      }
+    TORCH_CHECK_VALUE(!k || !overlap(q_out, *k_out), "rotary: the out tensors overlap");
   } else {
     q_out = fresh(q);
     if (k) k_out = fresh(*k);
@@ -576,6 +646,7 @@ PYBIND11_MODULE(_native, m) {
   m.def("add_rmsnorm_packed", &add_rmsnorm_packed, free());
   m.def("rmsnorm_packed_backward", &rmsnorm_packed_backward, free());
   m.def("rotary", &rotary, free());
+  m.def("overlap", &overlap, free());
   m.def("next_token_loss", &next_token_loss, free());
   m.def("scale_", &scale_, free());
   m.def("rotary_autograd", &rotary_autograd, free());

@@ -610,7 +610,7 @@ def rotary(q: torch.Tensor, k, positions: torch.Tensor, inv_freq=None, factor: f
     ``rotary_dim`` takes their sines and cosines from tables instead.  Both are multiplied by ``factor``.
     Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``; ``inverse`` applies the transpose (the
     backward pass).  ``out=(q_out, k_out)`` receives the results, for example K in a cache's slots; an output may
-    be its input itself (rotated in place) but may not overlap an input otherwise."""
+    be its input itself (rotated in place); outputs that overlap an input otherwise, or each other, are refused."""
     r = _lib.native().rotary(q, k, positions, inv_freq, factor, interleaved, inverse, out, tables, rotary_dim)
     _after("rotary")
     return r

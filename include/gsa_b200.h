@@ -335,8 +335,8 @@ int gsa_silu_mul(int dtype, int64_t T, int64_t n, const void* gu, int64_t gu_ld,
  * with the pairs (x_i, x_{i+rd/2}), or (x_{2i}, x_{2i+1}) when interleaved; inverse: s -> -s (the backward pass).
  * The other D - rd values are copied.
  *   q, k       gsa_rotary_side of [B, L, heads, D] tensors with contiguous values; strides in elements (input
- *              strides may be 0); in == out with the same strides rotates in place, otherwise the two must not
- *              overlap; k may be NULL.  At most 1024 heads together, D <= 1024.
+ *              strides may be 0); in == out with the same strides rotates in place, otherwise an output must not
+ *              overlap an input, nor the two outputs each other; k may be NULL.  At most 1024 heads together, D <= 1024.
  *   positions  int64, element (b, l) at b * pos_bstride + l * pos_lstride (0: shared)
  *   inv_freq   [rd/2] fp64 f_i, or NULL: c and s from cos_tab / sin_tab [tab_rows, >= rd/2] (row stride tab_ld,
  *              tab_dtype) times factor; a position outside the tables gives NaN and GSA_ERR_INDEX.
