@@ -43,6 +43,15 @@ def _fused(x: torch.Tensor, *params) -> bool:
     return not (torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in params)))
 
 
+def _plain(module: nn.Module, kind: type) -> bool:
+    """Whether calling ``module`` is kind.forward on its parameters and nothing else: no subclass or stand-in (an adapter, a
+    parametrization), no forward set on the instance, no hooks."""
+    return (type(module) is kind and "forward" not in vars(module)
+            and not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks
+                     or module._backward_pre_hooks or nn.modules.module._has_any_global_hook())
+            and not (kind is nn.Linear and module.bias is not None))
+
+
 class RMSNorm(nn.Module):
     """Root mean square layer normalisation (gsa_llama.py:18-30)."""
 
@@ -65,6 +74,15 @@ class RMSNorm(nn.Module):
             return ops.add_rmsnorm(residual, a, self.weight, self.eps)
         h = residual + a
         return h, self(h)
+
+
+def _packed_norm(norm: nn.Module, x: torch.Tensor, a: Optional[torch.Tensor] = None):
+    """(x + a, norm(x + a)), what the backward pass reads in 8 bits; by the module's own call where that is not a plain
+    RMSNorm's."""
+    if _plain(norm, RMSNorm):
+        return training.packed_add_rmsnorm(x, a, norm.weight, norm.eps)
+    h = x if a is None else x + a
+    return h, norm(h)
 
 
 class GSAMlp(nn.Module):
@@ -107,11 +125,16 @@ class GSADecoderLayer(nn.Module):
         self.packed_training = False  # under autograd: norm and MLP activations kept in 8 bits
 
     def _forward_packed(self, hidden_states, **attn):
-        n1, n2, mlp = self.input_layernorm, self.post_attention_layernorm, self.mlp
-        _, normed = training.packed_add_rmsnorm(hidden_states, None, n1.weight, n1.eps)
+        n2, mlp = self.post_attention_layernorm, self.mlp
+        normed = _packed_norm(self.input_layernorm, hidden_states)[1]
         attn_output, present_key_value, attn_weights = self.self_attn(normed, **attn)
-        out = training.packed_mlp_block(hidden_states, attn_output, n2.weight, mlp.gate_proj.weight,
-                                        mlp.up_proj.weight, mlp.down_proj.weight, n2.eps)
+        if _plain(n2, RMSNorm) and _plain(mlp, GSAMlp) and all(
+                _plain(p, nn.Linear) for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj)):
+            out = training.packed_mlp_block(hidden_states, attn_output, n2.weight, mlp.gate_proj.weight,
+                                            mlp.up_proj.weight, mlp.down_proj.weight, n2.eps)
+        else:
+            h, normed = _packed_norm(n2, hidden_states, attn_output)
+            out = h + mlp(normed)
         return out, present_key_value, attn_weights
 
     def forward(self, hidden_states: torch.Tensor, positions: Optional[torch.Tensor] = None,
@@ -184,7 +207,8 @@ class GSALlamaModel(nn.Module):
     def enable_packed_training(self, enabled: bool = True):
         """Under autograd, keep the norms' and the MLPs' activations in 8 bits for the backward pass: 33/32 bytes a
         value of h and of the MLP's (g, u), where the torch formulas keep some ten copies in 16 and 32 bits.  The
-        forward pass is not quantised; gradients are those at the kept values (within 2^-4 of the values each)."""
+        forward pass is not quantised; gradients are those at the kept values (within 2^-4 of the values each).  A norm or
+        an MLP that is replaced, wrapped or hooked is called as it is, its activations kept as torch keeps them."""
         self.packed_training = bool(enabled)
         for layer in self.layers:
             layer.packed_training = bool(enabled)
@@ -222,8 +246,8 @@ class GSALlamaModel(nn.Module):
                                                 output_attentions)
             presents.append(present)
             weights.append(attn)
-        if self.packed_training and not _fused(h, self.norm.weight):
-            h = training.packed_add_rmsnorm(h, None, self.norm.weight, self.norm.eps)[1]
+        if self.packed_training and not _fused(h, *self.norm.parameters()):
+            h = _packed_norm(self.norm, h)[1]
         else:
             h = self.norm(h)
         seen.append(h)

@@ -1,0 +1,125 @@
+"""The training-step operators in the modes that torch has beside plain reverse mode: adapters and hooks on a packed model's
+modules."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _randn(seed, *shape, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, device=DEV, generator=torch.Generator(device=DEV).manual_seed(seed)) * scale).to(dtype)
+
+
+# -- modules that are not what the packed path knows ---------------------------------------------
+class _Adapter(torch.nn.Module):
+    """base(x) + x A B, with base frozen."""
+
+    def __init__(self, base, rank=4):
+        super().__init__()
+        self.base = base.requires_grad_(False)
+        self.a = torch.nn.Parameter(torch.randn(base.in_features, rank, device=DEV) * 0.1)
+        self.b = torch.nn.Parameter(torch.randn(rank, base.out_features, device=DEV) * 0.1)
+
+    @property
+    def weight(self):
+        return self.base.weight
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a @ self.b
+
+
+class _LinearChild(torch.nn.Linear):
+    def forward(self, x):
+        return 2 * super().forward(x)
+
+
+def _model():
+    from gsa_b200 import GSAConfig, GSALlamaForCausalLM
+
+    cfg = GSAConfig(d_model=256, n_heads=4, n_kv_heads=2, d_indexer=32, n_indexer_heads=4, k_base=24, k_min=8, k_max=48,
+                    n_layers=2, d_ffn=512, vocab_size=384, max_position_embeddings=512)
+    torch.manual_seed(0)
+    return GSALlamaForCausalLM(cfg).to(DEV).train()
+
+
+def _bias(m):
+    mlp = m.model.layers[1].mlp
+    new = torch.nn.Linear(512, 256, bias=True, device=DEV)
+    with torch.no_grad():
+        new.weight.copy_(mlp.down_proj.weight)
+    mlp.down_proj = new
+
+
+def _child(m):
+    mlp = m.model.layers[0].mlp
+    new = _LinearChild(256, 512, bias=False, device=DEV)
+    with torch.no_grad():
+        new.weight.copy_(mlp.up_proj.weight)
+    mlp.up_proj = new
+
+
+def _instance_forward(m):
+    mlp = m.model.layers[1].mlp
+    plain = mlp.forward
+    mlp.forward = lambda x: 0.5 * plain(x)
+
+
+def _parametrization(m):
+    up = torch.nn.utils.parametrizations.weight_norm(m.model.layers[1].mlp.up_proj)
+    with torch.no_grad():
+        up.parametrizations.weight.original0.mul_(2)
+
+
+STANDINS = {
+    "adapter": lambda m: setattr(m.model.layers[0].mlp, "gate_proj", _Adapter(m.model.layers[0].mlp.gate_proj)),
+    "bias": _bias,
+    "subclass": _child,
+    "instance forward": _instance_forward,
+    "parametrization": _parametrization,
+    "hook on a projection": lambda m: m.model.layers[0].mlp.gate_proj.register_forward_hook(lambda mod, a, out: 2 * out),
+    "hook on the MLP": lambda m: m.model.layers[1].mlp.register_forward_pre_hook(lambda mod, a: (a[0] * 0.5,)),
+    "hook on the first norm": lambda m: m.model.layers[0].input_layernorm.register_forward_hook(lambda mod, a, out: 2 * out),
+    "hook on the second norm": lambda m: m.model.layers[0].post_attention_layernorm.register_forward_hook(
+        lambda mod, a, out: 2 * out),
+    "another last norm": lambda m: setattr(m.model, "norm", torch.nn.LayerNorm(256, device=DEV)),
+    "hook on the last norm": lambda m: m.model.norm.register_forward_hook(lambda mod, a, out: 2 * out),
+}
+
+
+@pytest.mark.parametrize("what", STANDINS)
+def test_packed_training_calls_what_is_there(cuda_ok, what):
+    """With a module replaced or hooked, a packed training step is the step without packing: the logits alike to fp32 rounding
+    through two layers, a gradient for the same parameters, and near it (a kept value is within 2^-4 and a term of a gradient
+    has at most four of them)."""
+    ids = torch.randint(0, 384, (2, 48), generator=torch.Generator().manual_seed(2)).to(DEV)
+    m = _model()
+    before = m(ids).logits.detach()
+    STANDINS[what](m)
+    got = []
+    for packed in (False, True):
+        m.enable_packed_training(packed)
+        m.zero_grad(set_to_none=True)
+        out = m(ids, labels=ids)
+        out.loss.backward()
+        got.append((out.logits.detach(), {n: p.grad.clone() for n, p in m.named_parameters() if p.grad is not None}))
+    (plain, ref), (logits, grads) = got
+    change = float((plain - before).norm())
+    assert change > 0  # the stand-in does something
+    # the sparse selection may differ in a row for a rounding's sake; the stand-in's own effect is far larger
+    assert float((logits - plain).norm()) < 0.01 * change
+    assert grads.keys() == ref.keys()
+    for name, g in grads.items():
+        assert float((g - ref[name]).norm()) <= 0.25 * float(ref[name].norm()), name
+
+
+def test_backward_hooks_fire(cuda_ok):
+    m = _model()
+    m.enable_packed_training()
+    seen = []
+    m.model.layers[0].mlp.register_full_backward_hook(lambda mod, gi, go: seen.append("mlp"))
+    m.model.layers[0].post_attention_layernorm.register_full_backward_pre_hook(lambda mod, go: seen.append("norm"))
+    ids = torch.randint(0, 384, (1, 32), generator=torch.Generator().manual_seed(2)).to(DEV)
+    m(ids, labels=ids).loss.backward()
+    assert sorted(seen) == ["mlp", "norm"]
