@@ -128,6 +128,7 @@ class GSADecoderLayer(nn.Module):
         n2, mlp = self.post_attention_layernorm, self.mlp
         normed = _packed_norm(self.input_layernorm, hidden_states)[1]
         attn_output, present_key_value, attn_weights = self.self_attn(normed, **attn)
+        attn_output = attn_output.to(hidden_states.dtype)  # under autocast its projections come in another
         if _plain(n2, RMSNorm) and _plain(mlp, GSAMlp) and all(
                 _plain(p, nn.Linear) for p in (mlp.gate_proj, mlp.up_proj, mlp.down_proj)):
             out = training.packed_mlp_block(hidden_states, attn_output, n2.weight, mlp.gate_proj.weight,

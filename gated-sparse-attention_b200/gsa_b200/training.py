@@ -136,7 +136,8 @@ def packed_add_rmsnorm(x: torch.Tensor, a: Optional[torch.Tensor], weight: torch
 class _PackedMlpBlock(torch.autograd.Function):
     """h = x + a, out = h + down(silu(gate(y)) * up(y)), y = RMSNorm(h) * weight.  Kept: h and (g, u) in 8 bits and
     the row statistics; y and silu(g) * u are formed again, by the kernels that run over the packed tensors
-    anyway, for the weight gradients."""
+    anyway, for the weight gradients.  Everything is computed in the tensors' type, autocast or not: its products in another
+    type would return the residual stream in that type, or meet kernels that take one type alone."""
 
     @staticmethod
     def forward(ctx, x, a, weight, w_gate, w_up, w_down, eps):
@@ -146,12 +147,14 @@ class _PackedMlpBlock(torch.autograd.Function):
         y2 = y.view(-1, d)
         n = w_gate.shape[0]
         gu = torch.empty(y2.shape[0], 2 * n, device=x.device, dtype=x.dtype)
-        torch.mm(y2, w_gate.t(), out=gu[:, :n])
-        torch.mm(y2, w_up.t(), out=gu[:, n:])
-        z, pgu = ops.silu_mul_packed(gu)
+        with torch.autocast("cuda", enabled=False):
+            torch.mm(y2, w_gate.t(), out=gu[:, :n])
+            torch.mm(y2, w_up.t(), out=gu[:, n:])
+            z, pgu = ops.silu_mul_packed(gu)
+            out = torch.addmm(h2, z, w_down.t()).view(x.shape)
         ctx.save_for_backward(ph.data, rstd, pgu.data, weight, w_gate, w_up, w_down)
         ctx.forms = (ph.shape, ph.dtype), (pgu.shape, pgu.dtype)
-        return torch.addmm(h2, z, w_down.t()).view(x.shape)
+        return out
 
     @staticmethod
     @once_differentiable
@@ -161,21 +164,23 @@ class _PackedMlpBlock(torch.autograd.Function):
         need = ctx.needs_input_grad
         d, n = w_gate.shape[1], w_gate.shape[0]
         do2 = d_out.reshape(-1, d)
-        dgu, z = ops.silu_mul_packed_backward(do2 @ w_down, PackedActivation(pgu, *form_gu), want_z=need[5])
-        d_down = do2.t() @ z if need[5] else None
-        dg, du = dgu[:, :n], dgu[:, n:]
-        dy = torch.addmm(dg @ w_gate, du, w_up)
-        dx, dw, y = ops.rmsnorm_packed_backward(dy.view(d_out.shape), PackedActivation(ph, *form_h), rstd, weight,
-                                                dh=d_out, want_y=need[3] or need[4], want_dw=need[2])
-        y2 = None if y is None else y.view(-1, d)
-        return (dx if need[0] else None, dx if need[1] else None, dw, dg.t() @ y2 if need[3] else None,
-                du.t() @ y2 if need[4] else None, d_down, None)
+        with torch.autocast("cuda", enabled=False):
+            dgu, z = ops.silu_mul_packed_backward(do2 @ w_down, PackedActivation(pgu, *form_gu), want_z=need[5])
+            d_down = do2.t() @ z if need[5] else None
+            dg, du = dgu[:, :n], dgu[:, n:]
+            dy = torch.addmm(dg @ w_gate, du, w_up)
+            dx, dw, y = ops.rmsnorm_packed_backward(dy.view(d_out.shape), PackedActivation(ph, *form_h), rstd, weight,
+                                                    dh=d_out, want_y=need[3] or need[4], want_dw=need[2])
+            y2 = None if y is None else y.view(-1, d)
+            return (dx if need[0] else None, dx if need[1] else None, dw, dg.t() @ y2 if need[3] else None,
+                    du.t() @ y2 if need[4] else None, d_down, None)
 
 
 def packed_mlp_block(x: torch.Tensor, a: Optional[torch.Tensor], weight: torch.Tensor, w_gate: torch.Tensor,
                      w_up: torch.Tensor, w_down: torch.Tensor, eps: float) -> torch.Tensor:
     """h + down(silu(gate(y)) * up(y)) with h = x + a (x when a is None) and y = RMSNorm(h) * weight: the second half of
-    a pre-norm decoder layer, keeping its activations in 8 bits for the backward pass."""
+    a pre-norm decoder layer, keeping its activations in 8 bits for the backward pass.  Tensors of one type, in which it is
+    computed also under torch.autocast."""
     return _PackedMlpBlock.apply(x, a, weight, w_gate, w_up, w_down, eps)
 
 

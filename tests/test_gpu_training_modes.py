@@ -1,5 +1,5 @@
 """The training-step operators in the modes that torch has beside plain reverse mode: adapters and hooks on a packed model's
-modules."""
+modules, autocast."""
 
 import pytest
 import torch
@@ -123,3 +123,49 @@ def test_backward_hooks_fire(cuda_ok):
     ids = torch.randint(0, 384, (1, 32), generator=torch.Generator().manual_seed(2)).to(DEV)
     m(ids, labels=ids).loss.backward()
     assert sorted(seen) == ["mlp", "norm"]
+
+
+# -- autocast -----------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_packed_mlp_block_under_autocast(cuda_ok, dtype):
+    """The block computes in its tensors' type whatever autocast says, forward and backward, inside its context or out."""
+    import gsa_b200 as gsa
+
+    rows, d, n = 24, 64, 96
+    shapes = ((rows, d), (rows, d), (d,), (n, d), (n, d), (d, n))
+    leaves = [_randn(i, *s, scale=s[-1] ** -0.5).requires_grad_(True) for i, s in enumerate(shapes)]
+    dout = _randn(9, rows, d)
+    out = gsa.packed_mlp_block(*leaves, 1e-5)
+    want = torch.autograd.grad(out, leaves, dout)
+    for inside in (False, True):
+        with torch.autocast("cuda", dtype=dtype):
+            got = gsa.packed_mlp_block(*leaves, 1e-5)
+            # the residual stream keeps its type: the next norm takes it
+            again = gsa.packed_add_rmsnorm(got, None, leaves[2], 1e-5)[1]
+            if inside:
+                grads = torch.autograd.grad(got, leaves, dout)
+        if not inside:
+            grads = torch.autograd.grad(got, leaves, dout)
+        assert got.dtype == again.dtype == torch.float32 and torch.equal(got, out)
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+
+def test_packed_training_under_autocast(cuda_ok):
+    """An fp32 model's packed step under bf16 autocast (its backward pass inside the context, as the attention's needs it): a gradient
+    for the same parameters as without packing, in their type, near it.  Kept values as above; the two differ by bf16 roundings in
+    the MLP beside that, of 2^-8 a product."""
+    ids = torch.randint(0, 384, (2, 48), generator=torch.Generator().manual_seed(2)).to(DEV)
+    got = []
+    for packed in (False, True):
+        m = _model()
+        m.enable_packed_training(packed)
+        with torch.autocast("cuda", dtype=torch.bfloat16):
+            out = m(ids, labels=ids)
+            out.loss.backward()
+        assert bool(torch.isfinite(out.loss))
+        got.append({n: p.grad for n, p in m.named_parameters() if p.grad is not None})
+    assert got[0].keys() == got[1].keys()
+    for name, g in got[1].items():
+        ref = got[0][name]
+        assert g.dtype == ref.dtype == torch.float32 and bool(torch.isfinite(g).all()), name
+        assert float((g - ref).norm()) <= (0.25 + 8 * 2.0 ** -8) * float(ref.norm()), name
