@@ -77,6 +77,14 @@ void alike(const optional<Tensor>& t, const Tensor& like) {
   if (t) alike(*t, like);
 }
 
+// A forward-mode tangent would be lost: none of the operators passes one on.
+void no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "forward-mode derivatives of the training-step operators are not implemented");
+}
+void no_tangent(const optional<Tensor>& t) {
+  if (t) no_tangent(*t);
+}
+
 void* ptr(const Tensor& t) { return t.data_ptr(); }
 void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
@@ -120,6 +128,7 @@ PackedRows packed_rows(const Tensor& data, int64_t rows, int64_t n) {
 
 Tensor pack(const Tensor& x) {
   on_gpu(x);
+  no_tangent(x);
   TORCH_CHECK_VALUE(x.dim() > 0, "pack_e4m3 takes a tensor with a last dimension");
   const int code = code_of(x.scalar_type());
   const int64_t n = x.size(-1), rows = rows_of(x.sizes());
@@ -147,6 +156,7 @@ Tensor unpack(const Tensor& data, const std::vector<int64_t>& shape, at::ScalarT
 
 std::tuple<Tensor, Tensor> silu_mul_packed(const Tensor& gu) {
   on_gpu(gu);
+  no_tangent(gu);
   TORCH_CHECK_VALUE(gu.dim() > 0 && gu.size(-1) % 2 == 0, "silu_mul_packed takes [..., 2n], got ", gu.sizes());
   const int code = code_of(gu.scalar_type());
   const int64_t n = gu.size(-1) / 2, rows = rows_of(gu.sizes());
@@ -164,6 +174,7 @@ std::tuple<Tensor, Tensor> silu_mul_packed(const Tensor& gu) {
 
 std::tuple<Tensor, optional<Tensor>> silu_mul_packed_backward(const Tensor& dz, const Tensor& data, bool want_z) {
   on_gpu(dz);
+  no_tangent(dz);
   beside(data, dz);
   TORCH_CHECK_VALUE(dz.dim() > 0, "silu_mul_packed_backward takes [..., n]");
   const int code = code_of(dz.scalar_type());
@@ -186,6 +197,9 @@ std::tuple<Tensor, optional<Tensor>> silu_mul_packed_backward(const Tensor& dz, 
 std::tuple<optional<Tensor>, Tensor, Tensor, Tensor> add_rmsnorm_packed(const Tensor& x, const optional<Tensor>& a,
                                                                         const Tensor& weight, double eps) {
   on_gpu(x);
+  no_tangent(x);
+  no_tangent(a);
+  no_tangent(weight);
   TORCH_CHECK_VALUE(x.dim() > 0 && x.size(-1) > 0 && weight.dim() == 1 && weight.size(0) == x.size(-1) &&
                         (!a || a->sizes() == x.sizes()),
                     "add_rmsnorm_packed: x ", x.sizes(), ", weight ", weight.sizes(),
@@ -214,6 +228,9 @@ std::tuple<Tensor, optional<Tensor>, optional<Tensor>> rmsnorm_packed_backward(c
                                                                                const optional<Tensor>& dh, bool want_y,
                                                                                bool want_dw) {
   on_gpu(dy);
+  no_tangent(dy);
+  no_tangent(weight);
+  no_tangent(dh);
   TORCH_CHECK_VALUE(dy.dim() > 0 && dy.size(-1) > 0 && weight.dim() == 1 && weight.size(0) == dy.size(-1) &&
                         (!dh || dh->sizes() == dy.sizes()) && rstd.sizes() == dy.sizes().slice(0, dy.dim() - 1) &&
                         rstd.scalar_type() == at::kFloat,
@@ -363,6 +380,9 @@ Tensor whole_positions(const Tensor& given, int64_t B, int64_t L) {
 // The checks that need no positions; angles made whole.
 void rotary_check(const Tensor& q, const optional<Tensor>& k, const Tensor& positions, Angles& a) {
   on_gpu(q);
+  no_tangent(q);
+  no_tangent(k);
+  no_tangent(a.inv_freq);
   alike(k, q);
   beside(positions, q);
   code_of(q.scalar_type());
@@ -548,6 +568,7 @@ std::tuple<optional<Tensor>, Tensor> add_rmsnorm_autograd(const Tensor& x, const
 std::tuple<Tensor, optional<Tensor>> next_token_loss(const Tensor& logits, const Tensor& labels_in, int64_t ignore_index,
                                                      bool want_grad) {
   on_gpu(logits);
+  no_tangent(logits);
   TORCH_CHECK_VALUE(logits.dim() == 3 && logits.size(2) > 0 && labels_in.dim() == 2 && labels_in.size(0) == logits.size(0) &&
                         labels_in.size(1) == logits.size(1),
                     "next_token_loss takes logits [B, L, V] and labels [B, L], got ", logits.sizes(), " and ",
@@ -572,6 +593,8 @@ std::tuple<Tensor, optional<Tensor>> next_token_loss(const Tensor& logits, const
 
 void scale_(const Tensor& x, const Tensor& factor) {
   on_gpu(x);
+  no_tangent(x);
+  no_tangent(factor);
   beside(factor, x);
   TORCH_CHECK_VALUE(x.is_contiguous() && factor.numel() == 1 && factor.scalar_type() == at::kFloat,
                     "scale_ takes a contiguous tensor and a one-element fp32 factor");

@@ -14,7 +14,8 @@ the backward pass, and the next-token loss with its gradient in one pass.
 
 The autograd functions are in csrc/torch_ops.cpp.  Each runs on its tensors' device and current stream and can be captured into a CUDA graph (a backward pass that is
 captured must not share its leaves with a graph of eager operations that is still alive: torch binds the leaves'
-accumulation to the stream of the first).  Second derivatives are not implemented.
+accumulation to the stream of the first).  Second derivatives and
+forward-mode ones are not implemented, and refused.
 """
 
 from __future__ import annotations

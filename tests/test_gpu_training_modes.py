@@ -1,5 +1,5 @@
 """The training-step operators in the modes that torch has beside plain reverse mode: adapters and hooks on a packed model's
-modules, autocast."""
+modules, autocast, forward-mode derivatives."""
 
 import pytest
 import torch
@@ -169,3 +169,42 @@ def test_packed_training_under_autocast(cuda_ok):
         ref = got[0][name]
         assert g.dtype == ref.dtype == torch.float32 and bool(torch.isfinite(g).all()), name
         assert float((g - ref).norm()) <= (0.25 + 8 * 2.0 ** -8) * float(ref.norm()), name
+
+
+# -- derivatives that there are not -------------------------------------------------------------
+def test_forward_mode_is_refused(cuda_ok):
+    """A tangent is not dropped in silence, whether or not anything requires a gradient."""
+    import gsa_b200 as gsa
+    from torch.autograd import forward_ad as fw
+
+    freq, _ = gsa.rotary_frequencies(16, device=DEV)
+    pos = torch.arange(6, device=DEV)
+    w = torch.ones(16, device=DEV)
+    lab = torch.zeros(2, 6, device=DEV, dtype=torch.long)
+    mats = [_randn(20 + i, *s) for i, s in enumerate(((8, 16), (8, 16), (16, 8)))]
+    calls = {
+        "rotary": lambda t: gsa.apply_rotary(t, None, pos, freq),
+        "rotary k": lambda t: gsa.apply_rotary(_randn(2, 2, 6, 2, 16), t, pos, freq),
+        "pack": lambda t: gsa.pack_activation(t),
+        "silu": lambda t: gsa.packed_silu_mul(t),
+        "norm": lambda t: gsa.packed_add_rmsnorm(t, None, w, 1e-5),
+        "norm addend": lambda t: gsa.packed_add_rmsnorm(_randn(3, 2, 6, 2, 16), t, w, 1e-5),
+        "block": lambda t: gsa.packed_mlp_block(t, None, w, *mats, 1e-5),
+        "loss": lambda t: gsa.fused_next_token_loss(t[:, :, 0], lab),
+    }
+    for name, call in calls.items():
+        for grad in (False, True):
+            x = _randn(1, 2, 6, 2, 16).requires_grad_(grad)
+            with fw.dual_level():
+                dual = fw.make_dual(x, torch.ones_like(x))
+                with pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                    call(dual)
+                with torch.no_grad(), pytest.raises((NotImplementedError, RuntimeError), match="forward|jvp"):
+                    call(dual)
+            call(x)  # and without one it is computed
+    x = _randn(1, 2, 6, 2, 16)
+    with fw.dual_level():
+        with pytest.raises(NotImplementedError, match="forward"):
+            gsa.packed_add_rmsnorm(x, None, fw.make_dual(w, torch.ones_like(w)), 1e-5)
+        with pytest.raises(NotImplementedError, match="forward"):
+            gsa.apply_rotary(x, None, pos, fw.make_dual(freq, torch.ones_like(freq)))
