@@ -98,10 +98,12 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     """(q', k'): q [B, L, H, D] and k [B, L, Hk, D] (or None) rotated to ``positions`` ([B, L], [1, L] or [L] integers)
     in the first ``2 * len(inv_freq)`` values of each head; the rest pass through.
 
-    ``inv_freq`` and ``attention_factor`` come from rotary_frequencies.  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1)
-    when ``interleaved``.  ``out=(q_out, k_out)`` (without autograd) receives the results: K straight into a
+    ``inv_freq`` and ``attention_factor`` come from rotary_frequencies and get no gradient (frequencies that want one are
+    refused).  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``.  ``out=(q_out, k_out)`` (without autograd) receives the results: K straight into a
     cache's slots (``store.kv[:, n:n + L, 0]``), or the inputs themselves to rotate in place; outputs that overlap an
     input otherwise, or each other, are refused."""
+    if torch.is_grad_enabled() and inv_freq.requires_grad:
+        raise NotImplementedError("apply_rotary gives no gradient for inv_freq; detach it")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         if out is not None:
             raise NotImplementedError("apply_rotary writes into given tensors without autograd only")

@@ -1,5 +1,5 @@
 """The training-step operators in the modes that torch has beside plain reverse mode: adapters and hooks on a packed model's
-modules, autocast, forward-mode derivatives."""
+modules, autocast, forward-mode derivatives, gradients that the operators do not give."""
 
 import pytest
 import torch
@@ -208,3 +208,19 @@ def test_forward_mode_is_refused(cuda_ok):
             gsa.packed_add_rmsnorm(x, None, fw.make_dual(w, torch.ones_like(w)), 1e-5)
         with pytest.raises(NotImplementedError, match="forward"):
             gsa.apply_rotary(x, None, pos, fw.make_dual(freq, torch.ones_like(freq)))
+
+
+def test_frequencies_have_no_gradient(cuda_ok):
+    """Frequencies that want a gradient are refused rather than left without one."""
+    import gsa_b200 as gsa
+
+    freq, _ = gsa.rotary_frequencies(16, device=DEV)
+    freq.requires_grad_(True)
+    pos = torch.arange(6, device=DEV)
+    for grad in (False, True):
+        q = _randn(1, 2, 6, 2, 16).requires_grad_(grad)
+        with pytest.raises(NotImplementedError, match="inv_freq"):
+            gsa.apply_rotary(q, None, pos, freq)
+        with torch.no_grad():
+            gsa.apply_rotary(q, None, pos, freq)
+        gsa.apply_rotary(q, None, pos, freq.detach())
