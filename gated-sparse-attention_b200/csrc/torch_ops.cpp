@@ -90,6 +90,11 @@ void* ptr(const optional<Tensor>& t) { return t ? t->data_ptr() : nullptr; }
 
 Tensor fresh(const Tensor& like) { return at::empty(like.sizes(), like.options()); }
 
+// A tensor that the caller hands in to be written: none whose own gradient would then be that of what it held before.
+void overwritable(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(at::GradMode::is_enabled() && t.requires_grad()),
+                              "the training-step operators write into tensors without autograd only");
+}
 // A tensor that the caller handed in has been written: graphs that saved it notice.
 void written(const Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -433,6 +438,8 @@ Pair rotary(const Tensor& q, const optional<Tensor>& k, const Tensor& positions,
     for (int i = 0; i < (k ? 2 : 1); ++i) {
       const Tensor &x = i ? *k : q, &o = i ? *k_out : q_out;
       alike(o, x);
+      no_tangent(o);
+      overwritable(o);
       TORCH_CHECK_VALUE(o.sizes() == x.sizes() && (o.size(3) <= 1 || o.stride(3) == 1) && (o.is_contiguous() || separate(o)),
                         "rotary: out tensors have their inputs' shape, contiguous values and no two elements in one place");
     }
@@ -595,6 +602,7 @@ void scale_(const Tensor& x, const Tensor& factor) {
   on_gpu(x);
   no_tangent(x);
   no_tangent(factor);
+  overwritable(x);
   beside(factor, x);
   TORCH_CHECK_VALUE(x.is_contiguous() && factor.numel() == 1 && factor.scalar_type() == at::kFloat,
                     "scale_ takes a contiguous tensor and a one-element fp32 factor");

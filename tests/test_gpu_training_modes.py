@@ -224,3 +224,26 @@ def test_frequencies_have_no_gradient(cuda_ok):
         with torch.no_grad():
             gsa.apply_rotary(q, None, pos, freq)
         gsa.apply_rotary(q, None, pos, freq.detach())
+
+
+def test_tensors_with_a_graph_are_not_overwritten(cuda_ok):
+    """Writing into a tensor that requires a gradient is refused while gradients are recorded, as torch's in-place operations
+    refuse a leaf; without recording it is done."""
+    import gsa_b200 as gsa
+
+    freq, _ = gsa.rotary_frequencies(16, device=DEV)
+    pos = torch.arange(6, device=DEV)
+    q, k = _randn(1, 2, 6, 2, 16), _randn(2, 2, 6, 2, 16)
+    leaf = torch.zeros_like(q).requires_grad_(True)
+    inner = leaf * 2
+    for outs in ((leaf, torch.empty_like(k)), (torch.empty_like(q), inner)):
+        with pytest.raises(NotImplementedError, match="without autograd"):
+            gsa.apply_rotary(q, k, pos, freq, out=outs)
+    for t in (leaf, inner):
+        assert bool((t.detach() == 0).all())
+        with pytest.raises(NotImplementedError, match="without autograd"):
+            gsa.ops.scale_(t, torch.full((1,), 2.0, device=DEV))
+    want = gsa.apply_rotary(q, None, pos, freq)[0]
+    with torch.no_grad():
+        gsa.apply_rotary(q, None, pos, freq, out=(leaf, None))
+    assert torch.equal(leaf.detach(), want)
