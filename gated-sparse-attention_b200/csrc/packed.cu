@@ -22,27 +22,38 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// 4 sigma(x) = 1 / ((1 + e^-x) / 4): the quarter keeps the reciprocal in the normal range for all e^-x that are, so that
-// x sigma(x) has its relative accuracy over the whole range (a plain fast reciprocal gives 0 under 2^-126).  e^-x is
-// 2^t times 2^lo with t = -x log2 e rounded and lo what that lost; beyond +-1e4 it is 0 or infinite in any case.
-__device__ __forceinline__ float sigmoid_times4(float x) {
+// sigma(x) = s k with k a power of two, s = 1 / ((1 + e^-x) k): k = 1/4 keeps the reciprocal in the normal range as long as e^-x
+// is in it.  Beyond (x < -87.3, where the 1 no longer counts) it is e^-x 2^-96 of which the reciprocal is taken, so that
+// x sigma(x), formed as (k x) s, has its relative accuracy down to the smallest normal number (x = -91.8; a plain fast
+// reciprocal gives 0 from -87.3 on).  e^-x is 2^t times 2^lo with t = -x log2 e rounded and lo what that lost; beyond +-1e4 it is 0
+// or infinite in any case.
+struct Sigmoid {
+  float s, k;
+};
+__device__ __forceinline__ Sigmoid sigmoid_of(float x) {
   constexpr float kLog2e = 1.44269502f, kLog2eLow = 1.925963e-8f, kLn2 = 0.693147181f;  // log2 e as a sum of two
   const float c = fminf(fmaxf(x, -1e4f), 1e4f);
   const float t = -c * kLog2e, lo = fmaf(-c, kLog2eLow, fmaf(-c, kLog2e, -t));
+  const bool far = t > 126.f;
   float e, r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(far ? t - 96.f : t));
   e *= fmaf(lo, kLn2, 1.0f);
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(fmaf(e, 0.25f, 0.25f)));
-  return r;
+  return {r, far ? 0x1p-98f : 0.25f};
 }
-__device__ __forceinline__ float silu_mul(float g, float u) { return 0.25f * g * sigmoid_times4(g) * u; }
+__device__ __forceinline__ float silu_mul(float g, float u) {
+  const Sigmoid q = sigmoid_of(g);
+  return q.k * g * q.s * u;
+}
 
 struct SwigluGrad {
   float dg, du, z;
 };
 __device__ __forceinline__ SwigluGrad swiglu_grad(float dz, float g, float u) {
-  const float s4 = sigmoid_times4(g), sig = 0.25f * s4, silu = 0.25f * g * s4;
-  return {dz * u * (sig * (1.0f + g * (1.0f - sig))), dz * silu, silu * u};
+  const Sigmoid q = sigmoid_of(g);
+  const float sig = q.k * q.s, silu = q.k * g * q.s;
+  // sig may be under the normal range, where silu carries the sum
+  return {dz * u * fmaf(silu, 1.0f - sig, sig), dz * silu, silu * u};
 }
 
 // A row is cut into 2 ceil(n / 32) halves of 16 values, one a thread, so that the two halves of a group are neighbouring
