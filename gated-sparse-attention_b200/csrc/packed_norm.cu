@@ -478,10 +478,11 @@ int gsa_add_rmsnorm_pack(int dtype, int64_t rows, int64_t d, const void* x, int6
             <<<(unsigned)((rows + per - 1) / per), kThreads, 0, s>>>(p);
       } else if (d <= kHalfRow) {
         add_rmsnorm_pack16_kernel<T, kRagged, false, 1, 512><<<row_grid, threads, 0, s>>>(p);
-      } else if (d <= kMaxRow && kRagged) {  // 32 values a thread would leave one CTA an SM
-        add_rmsnorm_pack16_kernel<T, kRagged, false, 1, 1024><<<row_grid, (unsigned)((d + 511) / 512 * 32), 0, s>>>(p);
       } else if (d <= kMaxRow) {
-        add_rmsnorm_pack16_kernel<T, false, false, 2, 512><<<row_grid, threads, 0, s>>>(p);
+        if constexpr (kRagged)  // 32 values a thread would leave one CTA an SM
+          add_rmsnorm_pack16_kernel<T, true, false, 1, 1024><<<row_grid, (unsigned)((d + 511) / 512 * 32), 0, s>>>(p);
+        else
+          add_rmsnorm_pack16_kernel<T, false, false, 2, 512><<<row_grid, threads, 0, s>>>(p);
       } else {
         add_rmsnorm_pack_long_kernel<T><<<row_grid, kThreads, 0, s>>>(p);
       }
