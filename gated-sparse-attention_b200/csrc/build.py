@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 CSRC = Path(__file__).resolve().parent
@@ -53,10 +54,30 @@ def _compile(nvcc: str, src: Path, obj: Path, verbose: bool, ptxas_v: bool) -> s
     return res.stderr if (verbose or ptxas_v) else ""
 
 
+def _native_for() -> str:
+    """What a compiled torch_ops.cpp is good for: the torch and the Python whose headers it has seen."""
+    import torch
+
+    return (f"torch {torch.__version__} {torch.version.git_version} cxx11abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)} "
+            f"python {sysconfig.get_config_var('SOABI')}")
+
+
+def _native_stale() -> bool:
+    built_for = OBJ_DIR / "native.txt"
+    changed = max(NATIVE_SRC.stat().st_mtime, (REPO / "include" / "gsa_b200.h").stat().st_mtime)
+    return (not NATIVE.exists() or NATIVE.stat().st_mtime < changed or not built_for.exists()
+            or built_for.read_text() != _native_for())
+
+
+def _build_native() -> None:
+    built_for = OBJ_DIR / "native.txt"
+    built_for.unlink(missing_ok=True)
+    _compile_native()
+    built_for.write_text(_native_for())
+
+
 def _compile_native() -> None:
     """_native.so: torch_ops.cpp against the installed torch's headers and libraries."""
-    import sysconfig
-
     import torch
 
     root = Path(torch.__file__).resolve().parent
@@ -80,9 +101,8 @@ def build(verbose: bool = False, ptxas_v: bool = False, force: bool = False) -> 
     jobs = []
     with cf.ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as ex:
         native = None
-        abi_time = max(NATIVE_SRC.stat().st_mtime, (REPO / "include" / "gsa_b200.h").stat().st_mtime)
-        if force or not NATIVE.exists() or NATIVE.stat().st_mtime < abi_time:
-            native = ex.submit(_compile_native)
+        if force or _native_stale():
+            native = ex.submit(_build_native)
         for src in srcs:
             obj = OBJ_DIR / (src.stem + ".o")
             stale = (force or not obj.exists() or obj.stat().st_mtime < src.stat().st_mtime
