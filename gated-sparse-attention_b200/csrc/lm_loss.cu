@@ -475,6 +475,8 @@ __global__ void __launch_bounds__(256) lm_loss_mean_kernel(const LossArgs a, int
   *a.loss = (float)(sum / (double)(parts ? a.ws->count : 0));
 }
 
+// x *= factor.  The gradient has been rounded to its type before its factor is known (the loss is formed first), so a factor that is
+// no power of two rounds it a second time: by up to a half step more in bf16 than a gradient formed with the factor.
 template <typename T>
 __global__ void __launch_bounds__(256) scale_kernel(int64_t n, T* x, const float* factor) {
   const float f = *factor;

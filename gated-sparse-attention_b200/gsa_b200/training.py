@@ -193,7 +193,9 @@ def packed_mlp_block(x: torch.Tensor, a: Optional[torch.Tensor], weight: torch.T
 def fused_next_token_loss(logits: torch.Tensor, labels: torch.Tensor, ignore_index: int = -100) -> torch.Tensor:
     """Mean cross entropy (fp32) of the token at t + 1 under logits[:, t]; labels of ``ignore_index`` do not count
     (NaN where none counts).  Under autograd the gradient is formed together with the loss, in one reading of the
-    logits, and handed out by the first backward pass (a second one through the same loss is refused)."""
+    logits, and handed out by the first backward pass (a second one through the same loss is refused).  A loss that is
+    scaled before its backward pass, such as ``loss / steps``, has that gradient read, multiplied and written once more, and
+    rounded once more unless the factor is a power of two."""
     if torch.is_grad_enabled() and logits.requires_grad:
         return _lib.native().loss_autograd(logits, labels, ignore_index)
     return ops.next_token_loss(logits, labels, ignore_index, want_grad=False)[0]

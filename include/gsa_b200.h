@@ -402,7 +402,7 @@ int gsa_rmsnorm_packed_backward(int dtype, int64_t rows, int64_t d, const void* 
  *   grad (nullable) [B, L, V] dtype = (softmax(x) - onehot(label)) / count; 0 in positions that do not count
  *   workspace  gsa_next_token_loss_workspace_size() bytes (the same for every size), 16-byte aligned
  * V <= 2^30.  Logits of -inf have probability 0.  A counted label outside [0, V) gives NaN and GSA_ERR_INDEX.
- * gsa_scale: x[0 .. n) *= *factor (a device scalar; 1 leaves x unread).
+ * gsa_scale: x[0 .. n) *= *factor (a device scalar; 1 leaves x unread), each product rounded to the dtype.
  */
 int gsa_next_token_loss(int dtype, int64_t B, int64_t L, int64_t V, const void* logits, int64_t x_bstride,
                         int64_t x_lstride, const int64_t* labels, int64_t lab_bstride, int64_t lab_lstride,

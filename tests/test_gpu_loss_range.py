@@ -138,3 +138,23 @@ def test_loss_of_labels_far_below(cuda_ok, dtype, nbytes):
     loss, grad = ops.next_token_loss(x, lab)
     want = (-2 * low + 4 * math.log(V)) / 5
     assert math.isfinite(float(loss)) and abs(float(loss) - want) <= 4 * U * want and bool(torch.isfinite(grad).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("factor", [1 / 3, 0.1, 1e-4, 7.0, -3.0, 0.0])
+def test_scaled_loss_is_rounded_twice_at_most(cuda_ok, dtype, factor):
+    """The gradient of a scaled loss is within the unscaled one's half step and one more of the exact one."""
+    import gsa_b200 as gsa
+
+    V, L = 1000, 40
+    logits = (torch.randn(1, L, V, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1)) * 3).to(dtype)
+    labels = torch.randint(0, V, (1, L), device=DEV, generator=torch.Generator(device=DEV).manual_seed(2))
+    want, grad, size, far = _oracle(logits[0, :-1], labels[0, 1:])
+    leaf = logits.clone().requires_grad_(True)
+    (gsa.fused_next_token_loss(leaf, labels) * factor).backward()
+    exact, size = grad * factor / (L - 1), size * abs(factor) / (L - 1)
+    half = torch.finfo(dtype).eps / 2
+    # two roundings to the type, the factor's own and the arithmetic's of the unscaled gradient (as for the rows above)
+    bound = (2 * half + 2 * half * half) * exact.abs() + size * ((V / 32 + 80) + 1.5 * far + 70) * U * (1 + 2 * half) + 2.0 ** -120
+    assert bool(((leaf.grad[0, :-1].double() - exact).abs() <= bound).all())
+    assert bool((leaf.grad[0, -1] == 0).all())
