@@ -48,7 +48,11 @@ def rotary_frequencies(dim: int, base: float = 10000.0, scaling: Optional[Dict[s
       "llama3"         frequencies of wavelength over original / low_freq_factor divided by factor, those under
                        original / high_freq_factor kept, linear in original / wavelength between
 
-    and its "attention_factor" (1 if absent) multiplies sines and cosines."""
+    and its "attention_factor" (1 if absent, for "yarn" too) multiplies sines and cosines.
+
+    The attention layer's own RotaryEmbedding gives the same angles for none, "ntk" and "yarn" under "type" only: any other
+    type leaves it at the standard frequencies (rope.py:53-57), and it reads neither "rope_type" nor "attention_factor".
+    Keys for a layer's cache are to be rotated with a dictionary that both read alike."""
     if dim < 2 or dim % 2:
         raise ValueError(f"rotary dim {dim} is not a positive even number")
     cfg = scaling or {}
