@@ -115,6 +115,8 @@ class GSAMlp(nn.Module):
 class GSADecoderLayer(nn.Module):
     """Pre-norm decoder layer: x + GSA(RMSNorm(x)), then h + MLP(RMSNorm(h)) (gsa_llama.py:49-112)."""
 
+    packed_training = False  # under autograd: norm and MLP activations kept in 8 bits (also of layers saved without the attribute)
+
     def __init__(self, config: GSAConfig, layer_idx: int):
         super().__init__()
         self.layer_idx = layer_idx
@@ -122,7 +124,6 @@ class GSADecoderLayer(nn.Module):
         self.self_attn = GatedSparseAttention(config)
         self.post_attention_layernorm = RMSNorm(config.d_model, eps=config.norm_eps)
         self.mlp = GSAMlp(config)
-        self.packed_training = False  # under autograd: norm and MLP activations kept in 8 bits
 
     def _forward_packed(self, hidden_states, **attn):
         n2, mlp = self.post_attention_layernorm, self.mlp
@@ -193,6 +194,8 @@ class GSALlamaModel(nn.Module):
     view of a buffer with headroom, and passing it back lets the next call append K, V and the
     indexer keys in place (``allocate_caches`` sizes them up front)."""
 
+    packed_training = False
+
     def __init__(self, config: GSAConfig):
         super().__init__()
         self.config = config
@@ -202,7 +205,6 @@ class GSALlamaModel(nn.Module):
         self.layers = nn.ModuleList([GSADecoderLayer(config, layer_idx=i) for i in range(config.n_layers)])
         self.norm = RMSNorm(config.d_model, eps=config.norm_eps)
         self.gradient_checkpointing = False
-        self.packed_training = False
         self._init_weights()
 
     def enable_packed_training(self, enabled: bool = True):
