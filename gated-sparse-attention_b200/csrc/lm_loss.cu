@@ -5,17 +5,18 @@
 //   grad = (softmax(x) - onehot(target)) / count, zero in the rows that do not count
 //
 // A CTA takes a row (a warp one of up to 4 KB, two to eight lanes one of up to 1 KB): its maximum and sum in one pass (online), then the gradient
-// from a second reading, which registers serve for short rows and the L2 for long ones: the rows in flight are up to
-// 76 MB.  So HBM sees each logit about once (1.1 times for rows of 250 KB) and each gradient value once.
+// from a second reading, which registers serve for short rows and the L2 for long ones, as far as it holds the rows in flight:
+// 48 to 97 MB for rows of up to 320 KB, 148 rows beyond (so rows of more than some 850 KB come from HBM twice).  HBM sees
+// each logit 1.24 times for rows of 250 KB, and each gradient value once; rows that do not count are not read at all.
 // Exponentials are 2^(x log2 e - M) by one multiply-add (two values an instruction) and one ex2, M the rounded m log2 e:
 // M is what the sums and the gradient share, so its rounding, a factor 2^r on all of them, cancels as long as 2^r does not
 // leave the range: |r| is half a step of M, 4 up to kFar.  A row whose |M| is larger (masked throughout with any value or
 // with -inf, or with a far largest one) is taken by differences first; beside a largest value within kFar, values under
 // kLow weigh 0 and are not met at all (a thread that has seen nothing else would be left with an r of its own of
 // any size).  Sums are in 32 bits within a row and in 64 across rows; each CTA adds its
-// rows in order and one CTA adds the CTAs' sums in order, so a loss is the same bits every time.  8192 x 128256 bf16: 0.70 to
-// 0.82 ms on different machines, 5.1 to 6.0 TB/s; what keeps it from a copy's 6.55 is latency between the two passes of a row
-// (no unit is more than two thirds busy).
+// rows in order and one CTA adds the CTAs' sums in order, so a loss is the same bits every time.  8192 x 128256 bf16, every
+// row counted: 0.79 ms, 5.4 TB/s; what keeps it from a copy's 6.55 is latency between the two passes of a row (no unit is busy
+// for more than about two thirds).  The forms with six pieces in flight and 64 to 256 threads a row spill 16 to 60 bytes a thread.
 #include <algorithm>
 
 #include "kernels.cuh"

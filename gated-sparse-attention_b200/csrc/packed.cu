@@ -10,8 +10,8 @@
 // a thread holds 16 neighbouring values (half a group, 32-byte loads and stores, one shuffle for the scale); where rows are
 // not whole multiples of that, or not aligned, through aligned pieces (kRagged: packed.cuh).  Whole rows run at HBM's rate (of
 // 6.55 TB/s for a copy): pack and unpack of 32768 x 4096 bf16 128 us, 6.4 TB/s; SwiGLU and its backward pass of 16384 x
-// 11008 0.50 ms, 6.5 TB/s.  Ragged ones are bound by instructions: 32768 x 4090 bf16 155 us (5.2 TB/s) and 0.53 ms (4.5); fp32
-// 16384 x 4090 124 us and 0.34 ms (5.4, 6.3).
+// 11008 0.50 ms, 6.5 TB/s.  Ragged ones are bound by instructions: 32768 x 4090 bf16 155 us (5.2 TB/s) and 0.55 ms (4.4); fp32
+// 16384 x 4090 124 us and 0.35 ms (5.4, 6.2).
 #include <algorithm>
 
 #include "packed.cuh"

@@ -12,7 +12,8 @@
 // warp one of up to 512 values (several, where rows are shorter still).  The backward pass keeps its CTAs for all rows:
 // each sums dw beside dx over its rows in order, and a last kernel adds the CTAs' sums in order.  32768 x 4096 bf16, forward and
 // backward: 0.383 ms, 6.3 TB/s (a copy runs at 6.55); x 4090, ragged and bound by instructions and, in the backward pass, by the 16
-// warps an SM that its registers leave: 0.67 ms, 3.6 TB/s.
+// warps an SM that its registers leave: 0.66 ms, 3.7 TB/s.  Whole fp32 rows of 513 to 8192 values spill 100 bytes a thread in the
+// backward pass, ragged fp32 ones over 8192 spill 56 (16384 x 4096 fp32: 0.19 ms against 0.17 of bytes).
 #include <algorithm>
 #include <type_traits>
 
@@ -435,8 +436,9 @@ int lanes_of(int64_t d) {
 }
 // Partial sums of dw: the CTAs of the backward kernel.  About 1024 threads an SM (the registers of more would not
 // fit); fewer where a CTA's rows one after another would be less than 8, down to two CTAs an SM, since a CTA's partial sums
-// cost what a row does (us for 3295 x 768 bf16 with 1, 2, 4, 8, 16 rows: 13.9, 12.5, 9.8, 11.4, 12.0; 2048 x 4096: 17.6, 17.5,
-// 17.5, 14.7, 14.8; 5374 x 530: 25.0, 25.0, 26.7, 26.2, 38.7).
+// cost what a row does.  us with at least 1, 2, 4, 8, 16 rows: 3295 x 768 bf16 13.9, 12.5, 9.8, 11.4, 12.0; 2048 x 4096 17.6, 17.5,
+// 17.5, 14.7, 14.8; 5374 x 530 25.0, 25.0, 26.7, 26.2, 38.7.  No number is the best of all three: 8 is within a sixth of each
+// size's best, 4 and fewer lose a fifth at the second or more at the first.
 int parts_of(int64_t rows, int64_t d) {
   if (d > kMaxRow) return (int)std::max<int64_t>(1, std::min<int64_t>(rows / 8, 128));
   const int64_t at_once = d <= kWarpRow ? kWarps * (32 / lanes_of(d)) : 1;  // rows of a CTA
