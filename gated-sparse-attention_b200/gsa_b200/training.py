@@ -14,8 +14,7 @@ the backward pass, and the next-token loss with its gradient in one pass.
 
 The autograd functions are in csrc/torch_ops.cpp.  Each runs on its tensors' device and current stream and can be captured into a CUDA graph (a backward pass that is
 captured must not share its leaves with a graph of eager operations that is still alive: torch binds the leaves'
-accumulation to the stream of the first).  Second derivatives and
-forward-mode ones are not implemented, and refused.
+accumulation to the stream of the first).  Second derivatives and forward-mode ones are not implemented, and refused.
 """
 
 from __future__ import annotations
@@ -103,9 +102,9 @@ def apply_rotary(q: torch.Tensor, k: Optional[torch.Tensor], positions: torch.Te
     in the first ``2 * len(inv_freq)`` values of each head; the rest pass through.
 
     ``inv_freq`` and ``attention_factor`` come from rotary_frequencies and get no gradient (frequencies that want one are
-    refused).  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``.  ``out=(q_out, k_out)`` (without autograd) receives the results: K straight into a
-    cache's slots (``store.kv[:, n:n + L, 0]``), or the inputs themselves to rotate in place; outputs that overlap an
-    input otherwise, or each other, are refused."""
+    refused).  Pairs are (i, i + rotary_dim/2), or (2i, 2i+1) when ``interleaved``.  ``out=(q_out, k_out)`` (without
+    autograd) receives the results: K straight into a cache's slots (``store.kv[:, n:n + L, 0]``), or the inputs themselves
+    to rotate in place; outputs that overlap an input otherwise, or each other, are refused."""
     if torch.is_grad_enabled() and inv_freq.requires_grad:
         raise NotImplementedError("apply_rotary gives no gradient for inv_freq; detach it")
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
